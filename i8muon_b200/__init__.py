@@ -2,11 +2,13 @@
 
 Drop-in names of the reference package (src/i8muon/__init__.py:1-5):
 ``Muon``, ``muon_step``, ``CutlassNSInt8``, ``recommend_coefficients``; plus ``FusedAdamW``, a
-companion for Muon's ``scalar_optimizer`` slot.
+companion for Muon's ``scalar_optimizer`` slot, and the layers whose gradients the two step on (``layers.py``).
 """
 from .adamw import FusedAdamW
 from .coefficients import recommend_coefficients
 from .engine import CutlassNSInt8, check_status
+from .layers import QuantisedActivation, layer_norm, quantise_activation, restore_activation
 from .optimizer import Muon, muon_step
 
-__all__ = ["Muon", "muon_step", "CutlassNSInt8", "recommend_coefficients", "check_status", "FusedAdamW"]
+__all__ = ["Muon", "muon_step", "CutlassNSInt8", "recommend_coefficients", "check_status", "FusedAdamW",
+           "layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]

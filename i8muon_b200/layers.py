@@ -1,0 +1,213 @@
+"""The layers around the matrices that Muon steps: what makes their gradients.
+
+``layer_norm``, and activations kept in eight bits for the backward pass (``quantise_activation``, ``restore_activation``,
+and the ``checkpoint=`` argument of the layers).  The functions take and return torch tensors, work on
+the current stream of the tensors' device without synchronising, and are differentiable once.  Each is one call into the
+sm_100a library forward and one backward; there is no fallback.  The reference starts at the gradient and has no counterpart.
+
+Eight-bit format: groups of 32 consecutive elements of a row share a power of two, the smallest 2^e with
+max|x| <= M 2^e (M = 127 for ``"int8"``, 448 for ``"fp8"``, E4M3; e >= -127), and each element is rounded to the nearest
+code, ties to even.  The values that codes stand for are exact in the activation's own type.  A group that holds an
+infinity or a NaN reads back as NaN.  An element costs 33/32 bytes.
+"""
+from __future__ import annotations
+
+from functools import lru_cache
+from typing import NamedTuple, Optional
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import native
+from .engine import on_device, raw_stream
+
+__all__ = ["layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]
+
+GROUP = 32
+_FORMATS = {None: native.EIGHT_NONE, "int8": native.EIGHT_INT8, "fp8": native.EIGHT_E4M3}
+_CODE_TYPES = {native.EIGHT_INT8: torch.int8, native.EIGHT_E4M3: torch.float8_e4m3fn}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+class QuantisedActivation(NamedTuple):
+    """An activation in eight bits: codes (..., 32 ceil(width / 32)) and exponent bytes (..., ceil(width / 32)) of a
+    tensor of ``shape`` and ``dtype``."""
+    codes: Tensor
+    exponents: Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+    checkpoint: str
+
+
+# ------------------------------------------------------------------ checks
+def _format(name, function):
+    try:
+        return _FORMATS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"{function}: checkpoint must be None, 'int8' or 'fp8'") from None
+
+
+@lru_cache(maxsize=None)
+def _is_sm100(index: int) -> bool:
+    return torch.cuda.get_device_capability(index)[0] == 10
+
+
+def _check_device(function, x, *others):
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{function}: all tensors must be on one device")
+    if not x.is_cuda:
+        raise ValueError(f"{function} needs CUDA tensors")
+    if not _is_sm100(x.device.index):
+        raise ValueError("The i8muon_b200 kernels are built for sm_100a (B200) only.")
+
+
+def _check_rows(function, x, dtypes=_FLOATS):
+    """``x`` as rows of its last dimension: (number of rows, width)."""
+    if not isinstance(x, Tensor) or x.ndim < 1:
+        raise ValueError(f"{function}: expected a tensor with at least one dimension")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{function}: the input must be " + " or ".join(str(t).replace("torch.", "") for t in dtypes))
+    width = x.shape[-1]
+    if width < 1:
+        raise ValueError(f"{function}: the last dimension must not be empty")
+    return x.numel() // width, width
+
+
+def _check_vector(function, name, v, width, dtype):
+    if v is not None and (not isinstance(v, Tensor) or v.shape != (width,) or v.dtype != dtype):
+        raise ValueError(f"{function}: {name} must be a vector of {width} elements of the input's type")
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _any_gradient(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------- activations in eight bits
+def _empty_codes(lead, width, device):
+    groups = -(-width // GROUP)
+    codes = torch.empty((*lead, groups * GROUP), dtype=torch.uint8, device=device)
+    return codes, torch.empty((*lead, groups), dtype=torch.uint8, device=device)
+
+
+def _quantise(x, rows, width, fmt, lead):
+    """Codes and exponents of a contiguous ``x``; its device must be current."""
+    codes, exponents = _empty_codes(lead, width, x.device)
+    if rows:
+        native.call("i8m_activation_quant", x.data_ptr(), native.torch_dtype_code(x.dtype), rows, width, fmt, codes.data_ptr(),
+                    exponents.data_ptr(), raw_stream(x.device.index))
+    return codes, exponents
+
+
+def quantise_activation(x: Tensor, checkpoint: str = "int8") -> QuantisedActivation:
+    """``x`` (float32, float16 or bfloat16, any number of rows of its last dimension) in eight bits.  Not
+    differentiable: the result carries no graph."""
+    fmt = _format(checkpoint, "quantise_activation")
+    if fmt == native.EIGHT_NONE:
+        raise ValueError("quantise_activation: checkpoint must be 'int8' or 'fp8'")
+    rows, width = _check_rows("quantise_activation", x)
+    _check_device("quantise_activation", x)
+    with on_device(x.device.index):
+        codes, exponents = _quantise(x.detach().contiguous(), rows, width, fmt, x.shape[:-1])
+    return QuantisedActivation(codes.view(_CODE_TYPES[fmt]), exponents, x.shape, x.dtype, checkpoint)
+
+
+def restore_activation(q: QuantisedActivation) -> Tensor:
+    """The values that ``q`` stands for, as a fresh tensor of the activation's shape and type."""
+    if not isinstance(q, QuantisedActivation):
+        raise ValueError("restore_activation: expected what quantise_activation returned")
+    fmt = _format(q.checkpoint, "restore_activation")
+    shape = torch.Size(q.shape)
+    if fmt == native.EIGHT_NONE or len(shape) < 1 or shape[-1] < 1 or q.dtype not in _FLOATS:
+        raise ValueError("restore_activation: not a quantised activation")
+    width = shape[-1]
+    groups = -(-width // GROUP)
+    if (q.codes.shape != (*shape[:-1], groups * GROUP) or q.codes.dtype != _CODE_TYPES[fmt]
+            or q.exponents.shape != (*shape[:-1], groups) or q.exponents.dtype != torch.uint8):
+        raise ValueError("restore_activation: codes and exponents do not belong to a tensor of this shape")
+    _check_device("restore_activation", q.codes, q.exponents)
+    device = q.codes.device
+    codes, exponents = q.codes.contiguous(), q.exponents.contiguous()
+    with on_device(device.index):
+        out = torch.empty(shape, dtype=q.dtype, device=device)
+        if out.numel():
+            native.call("i8m_activation_restore", codes.data_ptr(), exponents.data_ptr(), out.numel() // width, width, fmt,
+                        out.data_ptr(), native.torch_dtype_code(q.dtype), raw_stream(device.index))
+    return out
+
+
+# ------------------------------------------------------------------ layer norm
+def _norm_forward(x, weight, bias, eps, fmt, keep):
+    """(y, mean, rstd, codes, exponents) of a contiguous ``x``; the last four are None where nothing is kept."""
+    rows, width = x.numel() // x.shape[-1], x.shape[-1]
+    with on_device(x.device.index):
+        y = torch.empty_like(x)
+        mean = rstd = codes = exponents = None
+        if keep:
+            rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+            if fmt == native.EIGHT_NONE:
+                mean = torch.empty_like(rstd)
+            else:
+                codes, exponents = _empty_codes((rows,), width, x.device)
+        if rows:
+            native.call("i8m_layer_norm", x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd), _ptr(codes),
+                        _ptr(exponents), fmt if keep else native.EIGHT_NONE, rows, width, native.torch_dtype_code(x.dtype), eps,
+                        raw_stream(x.device.index))
+    return y, mean, rstd, codes, exponents
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, fmt):
+        x = x.contiguous()
+        weight = None if weight is None else weight.contiguous()
+        y, mean, rstd, codes, exponents = _norm_forward(x, weight, None if bias is None else bias.contiguous(), eps, fmt, True)
+        ctx.fmt, ctx.shape, ctx.dtype = fmt, x.shape, x.dtype
+        ctx.save_for_backward(x if fmt == native.EIGHT_NONE else None, mean, rstd, codes, exponents, weight)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, mean, rstd, codes, exponents, weight = ctx.saved_tensors
+        width = ctx.shape[-1]
+        rows = dy.numel() // width
+        dy = dy.contiguous()
+        with on_device(dy.device.index):
+            make = torch.zeros if rows == 0 else torch.empty
+            dx, dw, db = (make(shape, dtype=ctx.dtype, device=dy.device) if wanted else None
+                          for wanted, shape in zip(ctx.needs_input_grad, (ctx.shape, (width,), (width,))))
+            if rows and (dx is not None or dw is not None or db is not None):
+                size = native.layer_norm_scratch_bytes(rows, width) if dw is not None or db is not None else 0
+                scratch = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
+                native.call("i8m_layer_norm_backward", dy.data_ptr(), _ptr(x), _ptr(mean), rstd.data_ptr(), _ptr(codes),
+                            _ptr(exponents), ctx.fmt, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), rows, width,
+                            native.torch_dtype_code(ctx.dtype), _ptr(scratch), size, raw_stream(dy.device.index))
+        return dx, dw, db, None, None
+
+
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5, *,
+               checkpoint: Optional[str] = None) -> Tensor:
+    """Layer norm over the last dimension: ``(x - mean) / sqrt(var + eps) * weight + bias``.
+
+    ``x`` in float32, float16 or bfloat16; ``weight`` and ``bias`` (either may be None) are vectors of the same type.
+    Statistics and sums are FP32, the result is rounded once.  For the backward pass ``x`` and two statistics per row are
+    kept, or, with ``checkpoint="int8"`` or ``"fp8"``, the normalised rows in eight bits and one statistic; the gradients
+    are then those of the formula at the kept rows."""
+    fmt = _format(checkpoint, "layer_norm")
+    _, width = _check_rows("layer_norm", x)
+    _check_vector("layer_norm", "weight", weight, width, x.dtype)
+    _check_vector("layer_norm", "bias", bias, width, x.dtype)
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError("layer_norm: eps must be >= 0")
+    _check_device("layer_norm", x, weight, bias)
+    if _any_gradient(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps, fmt)
+    return _norm_forward(x.detach().contiguous(), None if weight is None else weight.contiguous(),
+                         None if bias is None else bias.contiguous(), eps, native.EIGHT_NONE, False)[0]

@@ -15,6 +15,7 @@ from functools import lru_cache
 from .build import LIBRARY
 
 F32, F16, BF16 = 0, 1, 2
+EIGHT_NONE, EIGHT_INT8, EIGHT_E4M3 = -1, 0, 1
 ROUTE_FLOAT, ROUTE_GRAM, ROUTE_INT8, ROUTE_BQ_INT8, ROUTE_BQ_FP8, ROUTE_INT8_FACTORED, ROUTE_INT8_CUBIC = range(7)
 
 
@@ -77,6 +78,12 @@ _SIGNATURES = {
                                c_float, c_float, _P]),
     "i8m_adamw": (c_int, [POINTER(_P), POINTER(_P), POINTER(_P), POINTER(_P), POINTER(c_longlong), c_int,
                           c_int, c_int, c_float, c_float, c_float, c_float, c_float, c_float, c_float, _P]),
+    "i8m_activation_quant": (c_int, [_P, c_int, c_longlong, c_int, c_int, _P, _P, _P]),
+    "i8m_activation_restore": (c_int, [_P, _P, c_longlong, c_int, c_int, _P, c_int, _P]),
+    "i8m_layer_norm": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_longlong, c_int, c_int, c_float, _P]),
+    "i8m_layer_norm_scratch_bytes": (c_int, [c_longlong, c_int, POINTER(c_size_t)]),
+    "i8m_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, c_int, _P, c_size_t,
+                                        _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -141,6 +148,13 @@ def ns_workspace_bytes(route, batch, rows, cols, dtype, compute, steps, fp16_fir
 def stats_scratch_bytes(batch, count) -> int:
     size = c_size_t(0)
     call("i8m_stats_scratch_bytes", batch, count, ctypes.byref(size))
+    return size.value
+
+
+@lru_cache(maxsize=1024)
+def layer_norm_scratch_bytes(rows, width) -> int:
+    size = c_size_t(0)
+    call("i8m_layer_norm_scratch_bytes", rows, width, ctypes.byref(size))
     return size.value
 
 

@@ -270,6 +270,38 @@ int i8m_adamw(void* const* params, const void* const* grads, float* const* exp_a
               int grad_dtype, float lr, float beta1, float beta2, float eps, float weight_decay,
               float bias_correction1, float bias_correction2, i8m_stream_t stream);
 
+/* ---- layers around the stepped matrices --------------------------------------
+ * The layers whose gradients the optimizer steps on.  No counterpart in the reference, which starts at the gradient.
+ *
+ * Activations in eight bits: groups of 32 consecutive elements of a row (the last one may be short) share an exponent e,
+ * the smallest integer >= -127 with max|x| <= M 2^e, M = 127 (INT8) or 448 (E4M3); a code is x 2^-e rounded to the
+ * nearest integer / E4M3 value, ties to even, and stands for code 2^e, which every dtype of x holds exactly
+ * (beside the largest number of a dtype, where rounding up would leave it, the code below is taken).
+ *   codes      rows x 32 ceil(width / 32) bytes, zero behind the width
+ *   exponents  rows x ceil(width / 32) bytes e + 127; 255 marks a group that holds an infinity or a NaN and reads back as
+ *              NaN throughout
+ * `format` of these functions is an i8m_eight_format; where it may be I8M_EIGHT_NONE the codes are not used. */
+enum i8m_eight_format { I8M_EIGHT_NONE = -1, I8M_EIGHT_INT8 = 0, I8M_EIGHT_E4M3 = 1 };
+int i8m_activation_quant(const void* x_device, int dtype, long long rows, int width, int format, void* codes_device,
+                         void* exponents_device, i8m_stream_t stream);
+int i8m_activation_restore(const void* codes_device, const void* exponents_device, long long rows, int width, int format,
+                           void* out_device, int dtype, i8m_stream_t stream);
+
+/* Layer norm over rows of `width` elements: u = (x - mean) rstd, rstd = 1 / sqrt(var + eps), y = u * weight + bias, all in
+ * FP32 and rounded once to `dtype`, the type of x, y, weight, bias and every gradient.
+ * weight, bias: NULL = ones, zeros.  mean, rstd: FP32 [rows] for the backward pass, or NULL.  format: I8M_EIGHT_NONE, or u is
+ * also written in eight bits (codes, exponents), which then serve the backward pass in the place of x and mean. */
+int i8m_layer_norm(const void* x_device, const void* weight_device, const void* bias_device, void* y_device, float* mean_device,
+                   float* rstd_device, void* codes_device, void* exponents_device, int format, long long rows, int width,
+                   int dtype, float eps, i8m_stream_t stream);
+/* Gradients of the above; dx, dweight, dbias may each be NULL.  scratch (only for dweight and dbias): partial sums over
+ * bands of rows, added up in a fixed order. */
+int i8m_layer_norm_scratch_bytes(long long rows, int width, size_t* bytes);
+int i8m_layer_norm_backward(const void* dy_device, const void* x_device, const float* mean_device, const float* rstd_device,
+                            const void* codes_device, const void* exponents_device, int format, const void* weight_device,
+                            void* dx_device, void* dweight_device, void* dbias_device, long long rows, int width, int dtype,
+                            void* scratch_device, size_t scratch_bytes, i8m_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,210 @@
+"""The layer operators against their formulas in 64 bits (layer_reference.py), through the public entry points."""
+import math
+
+import pytest
+import torch
+
+import layer_reference as ref
+from i8muon_b200 import layer_norm, quantise_activation, restore_activation
+
+pytestmark = pytest.mark.gpu
+TYPES = (torch.bfloat16, torch.float16, torch.float32)
+FORMATS = ("int8", "fp8")
+
+
+def normal(shape, seed, dtype, device, std=1.0, mean=0.0):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * std + mean).to(dtype).to(device)
+
+
+# ------------------------------------------------------------- eight-bit format
+@pytest.mark.parametrize("rows, width", [(1, 1), (3, 31), (2, 32), (5, 33), (7, 127), (4, 128), (1000, 96), (33, 1531), (129, 4096),
+                                         (1, 20000)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("checkpoint", FORMATS)
+def test_codes_stand_for_the_nearest_values_exactly(cuda_device, rows, width, dtype, checkpoint):
+    x = normal((rows, width), rows + width, torch.float64, "cpu")
+    x = (x * torch.exp2(torch.randint(-12, 6, (rows, width), generator=torch.Generator().manual_seed(3)).double())).to(dtype)
+    q = quantise_activation(x.to(cuda_device), checkpoint)
+    groups = -(-width // 32)
+    e, _ = ref.exponents_of(x.double(), checkpoint)
+    assert torch.equal(q.exponents.cpu().double(), e + 127)
+    assert q.codes.shape == (rows, 32 * groups) and q.exponents.shape == (rows, groups)
+    assert not q.codes.view(torch.uint8)[:, width:].any()
+    got = restore_activation(q)
+    assert got.dtype == dtype and got.shape == x.shape
+    assert torch.equal(got.cpu().double(), ref.kept(x.double(), checkpoint))   # a power of two: nothing is rounded twice
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("checkpoint", FORMATS)
+def test_groups_at_the_ends_of_the_range(cuda_device, dtype, checkpoint):
+    info = torch.finfo(dtype)
+    tiny = 2 * ref.TINY[dtype]
+    most = 127.0 if checkpoint == "int8" else 448.0
+    tops = [0.0, tiny, 3 * tiny, info.tiny, info.tiny * (2 - 2 * info.eps), most * 2.0 ** -10, most * 2.0 ** -10 * (1 + info.eps),
+            most / 2 * (1 + info.eps), info.max, info.max / 2, 1.0, 2.0 - info.eps * 2]
+    rows = torch.zeros(len(tops), 32, dtype=torch.float64)
+    for i, top in enumerate(tops):
+        rows[i] = torch.linspace(-1, 1, 32, dtype=torch.float64) * top
+        rows[i, 7] = -top
+    x = rows.to(dtype)
+    assert torch.isfinite(x).all()
+    got = restore_activation(quantise_activation(x.to(cuda_device), checkpoint)).cpu()
+    assert torch.isfinite(got).all()
+    want = ref.kept(x.double(), checkpoint, dtype=dtype)
+    assert torch.equal(got.double(), want)
+    # half a step: top / 127 of the group for INT8, 2^-4 of the value or 2^-10 of the scale for E4M3, 2^-128 at the lowest
+    # scale; a whole step where the code below is taken
+    off, top = (got.double() - x.double()).abs(), x.double().abs().amax(1, keepdim=True)
+    bound = top / 127 if checkpoint == "int8" else torch.maximum(x.double().abs() * 2.0 ** -4, top / 224 * 2.0 ** -10)
+    whole = 1 + (top > info.max / 2).double()
+    assert (off <= bound * whole + 2.0 ** -128).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("checkpoint", FORMATS)
+@pytest.mark.parametrize("width", [64, 97])
+def test_a_group_that_is_not_finite_reads_back_as_nan(cuda_device, dtype, checkpoint, width):
+    x = normal((4, width), 5, dtype, cuda_device)
+    x[0, 3], x[1, 40], x[2, 63] = math.inf, -math.inf, math.nan
+    got = restore_activation(quantise_activation(x, checkpoint))
+    want = torch.zeros_like(x, dtype=torch.bool)
+    want[0, :32] = want[1, 32:64] = want[2, 32:64] = True
+    assert torch.equal(torch.isnan(got), want)
+    clean = torch.where(want, torch.zeros_like(x), x).cpu().double()
+    assert torch.equal(got.cpu().double()[~want.cpu()], ref.kept(clean, checkpoint)[~want.cpu()])
+
+
+def test_shapes_strides_and_offsets(cuda_device):
+    base = normal((6, 5, 70), 7, torch.bfloat16, cuda_device)
+    for x in (base, base.transpose(0, 1), base[..., 1:], base[:, ::2, 3:67], base.reshape(-1)[1:2001].view(20, 100), base[0, 0],
+              base[:, :0], base[0, 0, :1].expand(9, 64)):
+        got = restore_activation(quantise_activation(x, "int8"))
+        want = ref.kept(x.reshape(-1, x.shape[-1]).cpu().double(), "int8").reshape(x.shape)
+        assert got.shape == x.shape and torch.equal(got.cpu().double(), want)
+    x = base.clone().requires_grad_()
+    assert not quantise_activation(x, "fp8").exponents.requires_grad
+
+
+# ------------------------------------------------------------------ layer norm
+WIDTHS = [1, 2, 31, 33, 96, 128, 768, 1000, 1024, 1531, 2048, 4096, 6144, 8192, 8200, 16384, 20001]
+
+
+def norm_inputs(rows, width, dtype, device, affine, shift):
+    x = normal((rows, width), width, dtype, device, 1.0, shift)
+    w = normal((width,), 1, dtype, device, 0.1, 1.0) if affine[0] else None
+    b = normal((width,), 2, dtype, device, 0.1) if affine[1] else None
+    return x, w, b, normal((rows, width), 3, dtype, device)
+
+
+def double(t):
+    return None if t is None else t.detach().double()
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, affine, shift", [(5, (True, True), 0.0), (301, (True, False), 3.0), (1, (False, False), -0.5)])
+def test_layer_norm_and_its_gradients(cuda_device, width, dtype, rows, affine, shift):
+    eps = 1e-5
+    x, w, b, dy = norm_inputs(rows, width, dtype, cuda_device, affine, shift)
+    leaves = [t.requires_grad_() for t in (x, w, b) if t is not None]
+    y = layer_norm(x, w, b, eps)
+    got = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        assert torch.equal(layer_norm(x, w, b, eps), y)        # the same values where nothing is kept
+    want, tol, u, tol_u, rstd, rel = ref.layer_norm(double(x), double(w), double(b), eps, dtype)
+    ref.assert_within(y, want, tol, "y")
+    wants = ref.layer_norm_gradients(double(dy), u, tol_u, rstd, rel, double(w), dtype)
+    for name, g in zip([n for n, t in (("dx", x), ("dw", w), ("db", b)) if t is not None], got):
+        assert g.dtype == dtype
+        ref.assert_within(g, *wants[name], name)
+
+
+@pytest.mark.parametrize("rows, width", [(1, 1), (40, 33), (300, 768), (17, 1531), (64, 4096), (9, 8192), (5, 16384), (3, 20001)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("checkpoint", FORMATS)
+def test_layer_norm_gradients_at_rows_kept_in_eight_bits(cuda_device, rows, width, dtype, checkpoint):
+    eps = 1e-5
+    x, w, b, dy = norm_inputs(rows, width, dtype, cuda_device, (True, True), 1.0 if width > 1 else 0.0)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = layer_norm(x, w, b, eps, checkpoint=checkpoint)
+    got = torch.autograd.grad(y, leaves, dy)
+    assert torch.equal(y, layer_norm(x, w, b, eps))
+    _, _, u, tol_u, rstd, rel = ref.layer_norm(double(x), double(w), double(b), eps, dtype)
+    kept, off = ref.kept_with_slack(u, tol_u, checkpoint)
+    wants = ref.layer_norm_gradients(double(dy), kept, off, rstd, rel, double(w), dtype)
+    for name, g in zip(("dx", "dw", "db"), got):
+        ref.assert_within(g, *wants[name], name)
+
+
+def test_layer_norm_gradients_against_differences(cuda_device):
+    """Central differences of the formula in 64 bits: (f(t + h) - f(t - h)) / 2h is off by h^2 f''' / 6 and by the
+    rounding of f over h, both below 1e-6 here; the FP32 gradients by their own bounds, a few 1e-6."""
+    x, w, b, dy = norm_inputs(3, 40, torch.float32, cuda_device, (True, True), 0.5)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    got = torch.autograd.grad(layer_norm(x, w, b, 1e-3), leaves, dy)
+
+    def f(*ts):
+        x, w, b = ts
+        c = x - x.mean(1, keepdim=True)
+        return ((c / torch.sqrt(c.square().mean(1, keepdim=True) + 1e-3) * w + b) * double(dy)).sum()
+    args = [double(t) for t in leaves]
+    h = 1e-4
+    for k, t in enumerate(args):
+        for i in range(0, t.numel(), 7):
+            side = []
+            for sign in (1, -1):
+                moved = [a.clone() for a in args]
+                moved[k].view(-1)[i] += sign * h
+                side.append(f(*moved).item())
+            assert abs((side[0] - side[1]) / (2 * h) - got[k].reshape(-1)[i].item()) < 1e-5
+
+
+def test_layer_norm_takes_any_strides_and_leading_dimensions(cuda_device):
+    base = normal((4, 6, 70), 1, torch.bfloat16, cuda_device)
+    for x in (base.transpose(0, 1), base[..., 1:65], base[:, ::3], base[0, 0], base.reshape(-1)[3:3 + 640].view(10, 64),
+              base[0, :1].expand(5, 70)):
+        w = normal((2 * x.shape[-1],), 2, torch.bfloat16, cuda_device)[::2]
+        leaf = x.detach().requires_grad_()
+        y = layer_norm(leaf, w)
+        flat = x.reshape(-1, x.shape[-1]).double()
+        want, tol, u, tol_u, rstd, rel = ref.layer_norm(flat, double(w), None, 1e-5, torch.bfloat16)
+        assert y.shape == x.shape
+        ref.assert_within(y.reshape(flat.shape), want, tol, "y")
+        dy = normal(tuple(reversed(y.shape)), 3, torch.bfloat16, cuda_device).permute(*reversed(range(y.ndim)))
+        dx, = torch.autograd.grad(y, leaf, dy)
+        wants = ref.layer_norm_gradients(dy.reshape(flat.shape).double(), u, tol_u, rstd, rel, double(w), torch.bfloat16)
+        ref.assert_within(dx.reshape(flat.shape), *wants["dx"], "dx")
+
+
+def test_layer_norm_edges(cuda_device):
+    # no rows: empty result, zero gradients of the vectors
+    w, b = torch.ones(8, device=cuda_device, requires_grad=True), torch.zeros(8, device=cuda_device, requires_grad=True)
+    x = torch.zeros(0, 8, device=cuda_device, requires_grad=True)
+    for checkpoint in (None, "int8"):
+        dx, dw, db = torch.autograd.grad(layer_norm(x, w, b, checkpoint=checkpoint).sum(), (x, w, b))
+        assert dx.shape == (0, 8) and not dw.any() and not db.any()
+    # constant rows: variance zero
+    x = torch.full((2, 8), 3.0, device=cuda_device, requires_grad=True)
+    y = layer_norm(x, w, b)
+    assert not y.any()
+    dx, = torch.autograd.grad(y, x, torch.randn(2, 8, device=cuda_device))
+    assert torch.isfinite(dx).all()
+    # a row that is not finite spoils itself alone
+    x = normal((3, 64), 1, torch.float32, cuda_device)
+    x[1, 5] = math.inf
+    y = layer_norm(x)
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2]).all()
+    # values far from zero: the variance is taken around the mean
+    x = normal((4, 1024), 2, torch.float32, cuda_device, 1.0, 1000.0)
+    want, tol, *_ = ref.layer_norm(x.double(), None, None, 1e-5, torch.float32)
+    ref.assert_within(layer_norm(x), want, tol, "y")
+    # only what is asked for is computed, and the backward pass is differentiable once
+    x = normal((3, 64), 1, torch.float32, cuda_device).requires_grad_()
+    w = torch.ones(64, device=cuda_device, requires_grad=True)
+    dw, = torch.autograd.grad(layer_norm(x.detach(), w).sum(), w)
+    assert dw.shape == (64,)
+    dx, = torch.autograd.grad(layer_norm(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
