@@ -7,8 +7,8 @@ companion for Muon's ``scalar_optimizer`` slot, and the layers whose gradients t
 from .adamw import FusedAdamW
 from .coefficients import recommend_coefficients
 from .engine import CutlassNSInt8, check_status
-from .layers import QuantisedActivation, layer_norm, quantise_activation, restore_activation
+from .layers import QuantisedActivation, layer_norm, linear, quantise_activation, restore_activation
 from .optimizer import Muon, muon_step
 
 __all__ = ["Muon", "muon_step", "CutlassNSInt8", "recommend_coefficients", "check_status", "FusedAdamW",
-           "layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]
+           "linear", "layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]

@@ -42,6 +42,38 @@ int eight_restore(const void* codes, const void* exponents, long long rows, int 
   return 0;
 }
 
+int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width, int pitch, cudaStream_t stream) {
+  const unsigned grid = unsigned(std::min<long long>((rows * (pitch / 8) + 255) / 256, 148LL * 16));
+  if (dtype == I8M_F16)
+    launch(pitch_rows_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(src), static_cast<__half*>(dst), rows, width, pitch);
+  else
+    launch(pitch_rows_kernel<__nv_bfloat16>, grid, 256, 0, stream, static_cast<const __nv_bfloat16*>(src),
+           static_cast<__nv_bfloat16*>(dst), rows, width, pitch);
+  LAUNCH_CHECK("pitch_rows");
+  return 0;
+}
+
+template <typename E>
+static int linear_dz_typed(const LinearDz& d, cudaStream_t stream) {
+  const int bands = row_bands(d.rows);
+  const PreActivation<E> kept{static_cast<const E*>(d.z), static_cast<const uint8_t*>(d.codes),
+                              static_cast<const uint8_t*>(d.exponents), d.z_pitch, eight_groups(d.width)};
+  auto kernel = d.format == EIGHT_INT8 ? linear_dz_kernel<E, EIGHT_INT8>
+              : d.format == EIGHT_E4M3 ? linear_dz_kernel<E, EIGHT_E4M3> : linear_dz_kernel<E, -1>;
+  launch(kernel, dim3(cdiv(d.width, 32), bands), 32 * COLUMN_LANES, 0, stream, static_cast<const E*>(d.dy), kept,
+         static_cast<E*>(d.dz), d.db ? d.partials : nullptr, d.rows, d.width, d.dz_pitch, (d.rows + bands - 1) / bands, d.activation);
+  LAUNCH_CHECK("linear_dz");
+  if (d.db) {
+    launch(column_fold_kernel<E>, cdiv(d.width, 32), 32 * COLUMN_LANES, 0, stream, d.partials, static_cast<E*>(d.db),
+           static_cast<E*>(nullptr), d.width, bands);
+    LAUNCH_CHECK("column_fold");
+  }
+  return 0;
+}
+int linear_dz(const LinearDz& d, cudaStream_t stream) {
+  return d.dtype == I8M_F16 ? linear_dz_typed<__half>(d, stream) : linear_dz_typed<__nv_bfloat16>(d, stream);
+}
+
 }  // namespace i8m
 
 // ================================================================== eight-bit activations

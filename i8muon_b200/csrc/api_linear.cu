@@ -1,0 +1,184 @@
+// C ABI: linear layers (product with bias, activation and residual in the epilogue) and their backward pass.
+#include "launch_gemm.cuh"
+#include "epi_linear.cuh"
+#include "layers.cuh"
+
+using namespace i8m;
+
+namespace {
+
+// An operand: `extent` rows along K, or (mn) K rows along its extent; rows `pitch` elements apart.
+struct Operand {
+  const void* p;
+  int pitch, mn;
+};
+
+// out (m, n) = a b^T over k.
+template <typename E>
+int product(const Operand& a, const Operand& b, int m, int n, int k, const LinearArgs& args, unsigned* status, cudaStream_t stream,
+            const char* name) {
+  using Epi = EpiLinear<E>;
+  GemmGeom g{};
+  g.batch = 1; g.m = g.lm = m; g.n = g.ln = n; g.k = k;
+  g.tiles_m = cdiv(m, TILE); g.tiles_n = cdiv(n, TILE);
+  const long long tiles = (long long)g.tiles_m * g.tiles_n;
+  if (tiles > 0x7fffffffLL) return fail(I8M_E_LIMIT, "%s: too many tiles", name);
+  g.tiles_per_batch = int(tiles);
+  g.num_kb = cdiv(2LL * k, 128);
+  g.debug_simt = g_starve_producers ? 0x100 : 0;
+  g.a_mn = a.mn; g.b_mn = b.mn;
+  g.group = wide_group(2LL * k);
+  g.a_raw = a.p; g.b_raw = b.p; g.status = status;
+  CUtensorMap ma, mb;
+  if (int rc = make_operand_map(&ma, a.p, 2, k, m, 1, a.mn, a.pitch)) return rc;
+  if (int rc = make_operand_map(&mb, b.p, 2, k, n, 1, b.mn, b.pitch)) return rc;
+  constexpr size_t SMEM = wholek_wide_smem_bytes<Epi>();
+  auto kernel = wholek_wide_kernel<Epi>;
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(allowed, kernel, SMEM)) return rc;
+  const long long pairs = wide_units_per_batch(g.tiles_m, g.tiles_n, 0);
+  g.narrow = narrow_units(tiles, pairs, g.num_kb, sm_count());
+  launch(kernel, unsigned(std::min<long long>(g.narrow ? tiles : pairs, sm_count())), WKW_THREADS, SMEM, stream, ma, mb, g, args);
+  LAUNCH_CHECK(name);
+  return 0;
+}
+template <typename... A>
+int product_of(int dtype, A&&... args) {
+  return dtype == I8M_F16 ? product<__half>(std::forward<A>(args)...) : product<__nv_bfloat16>(std::forward<A>(args)...);
+}
+
+bool addressable(const void* p, int width) { return width % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_linear(const char* name, int rows, int inner, int outer, int dtype, int activation, int format) {
+  if (rows < 1 || inner < 1 || outer < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
+  if (dtype != I8M_F16 && dtype != I8M_BF16) return fail(I8M_E_ARGUMENT, "%s: dtype must be a 16-bit type", name);
+  if (activation < 0 || activation >= ACTIVATIONS) return fail(I8M_E_ARGUMENT, "%s: bad activation %d", name, activation);
+  if (format < -1 || format > EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
+  if (inner > MAX_LAYER_WIDTH || outer > MAX_LAYER_WIDTH || rows > MAX_LAYER_ROWS)
+    return fail(I8M_E_LIMIT, "%s: %d rows, %d x %d weights are above the limits", name, rows, outer, inner);
+  return 0;
+}
+
+// Workspace: pieces one behind the other, each aligned to 256 bytes.
+struct Carver {
+  uint8_t* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base + used;
+    used += align256(bytes);
+    return p;
+  }
+};
+size_t rows_bytes(long long rows, int pitch) { return size_t(rows) * pitch * 2; }
+
+// What a forward or backward call copies or computes into its workspace.
+struct ForwardPieces {
+  void *x = nullptr, *w = nullptr;
+  size_t bytes;
+  ForwardPieces(void* base, const void* x_in, const void* w_in, int rows, int inner, int outer) {
+    Carver c{static_cast<uint8_t*>(base)};
+    const int pitch = pad_to(inner, 8);
+    if (!addressable(x_in, inner)) x = c.take(rows_bytes(rows, pitch));
+    if (!addressable(w_in, inner)) w = c.take(rows_bytes(outer, pitch));
+    bytes = c.used;
+  }
+};
+struct BackwardPieces {
+  void *w = nullptr, *x = nullptr, *dz = nullptr;
+  float* partials = nullptr;
+  size_t bytes;
+  BackwardPieces(void* base, const void* dy, const void* x_in, const void* w_in, int rows, int inner, int outer, int activation,
+                 int format, bool dx, bool dw, bool db) {
+    Carver c{static_cast<uint8_t*>(base)};
+    const int pitch = pad_to(inner, 8);
+    if (dx && !addressable(w_in, inner)) w = c.take(rows_bytes(outer, pitch));
+    if (dw && (format >= 0 || !addressable(x_in, inner))) x = c.take(rows_bytes(rows, pitch));
+    if ((dx || dw) && (activation != ACT_NONE || !addressable(dy, outer))) dz = c.take(rows_bytes(rows, pad_to(outer, 8)));
+    if (db) partials = static_cast<float*>(c.take(size_t(row_bands(rows)) * 2 * outer * sizeof(float)));
+    bytes = c.used;
+  }
+};
+
+}  // namespace
+
+extern "C" int i8m_linear_workspace_bytes(const void* x, const void* weight, int rows, int inner, int outer, size_t* bytes) {
+  if (!bytes) return fail(I8M_E_ARGUMENT, "linear_workspace_bytes: null pointer");
+  if (int rc = check_linear("linear_workspace_bytes", rows, inner, outer, I8M_BF16, 0, -1)) return rc;
+  *bytes = ForwardPieces(nullptr, x, weight, rows, inner, outer).bytes;
+  return 0;
+}
+extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z,
+                          void* z_codes, void* z_exponents, int format, int activation, int rows, int inner, int outer, int dtype,
+                          void* workspace, size_t workspace_bytes, uint32_t* status, i8m_stream_t stream) {
+  if (!x || !weight || !y || !status) return fail(I8M_E_ARGUMENT, "linear: null pointer");
+  if (int rc = check_linear("linear", rows, inner, outer, dtype, activation, format)) return rc;
+  if (format >= 0 && !z_codes != !z_exponents) return fail(I8M_E_ARGUMENT, "linear: codes without exponents");
+  if ((reinterpret_cast<uintptr_t>(z) | (format >= 0 ? reinterpret_cast<uintptr_t>(z_codes) : 0)) & 15u)
+    return fail(I8M_E_ARGUMENT, "linear: z or its codes are not 16-byte aligned");
+  const ForwardPieces pieces(workspace, x, weight, rows, inner, outer);
+  if (pieces.bytes && (!workspace || workspace_bytes < pieces.bytes))
+    return fail(I8M_E_WORKSPACE, "linear: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, pieces.bytes);
+  const int pitch = pad_to(inner, 8);
+  if (pieces.x) { if (int rc = pitch_rows(x, pieces.x, dtype, rows, inner, pitch, S(stream))) return rc; }
+  if (pieces.w) { if (int rc = pitch_rows(weight, pieces.w, dtype, outer, inner, pitch, S(stream))) return rc; }
+  LinearArgs a{};
+  a.y = y; a.bias = bias; a.residual = residual;
+  a.z = format < 0 ? z : nullptr; a.z_pitch = pad_to(outer, 8);
+  a.codes = format >= 0 ? static_cast<uint8_t*>(z_codes) : nullptr; a.exponents = static_cast<uint8_t*>(z_exponents);
+  a.groups = eight_groups(outer); a.format = format; a.activation = activation;
+  return product_of(dtype, Operand{pieces.x ? pieces.x : x, pitch, 0}, Operand{pieces.w ? pieces.w : weight, pitch, 0}, rows, outer,
+                    inner, a, status, S(stream), "linear");
+}
+
+extern "C" int i8m_linear_backward_workspace_bytes(const void* dy, const void* x, const void* weight, int rows, int inner, int outer,
+                                                   int activation, int format, int dx, int dweight, int dbias, size_t* bytes) {
+  if (!bytes) return fail(I8M_E_ARGUMENT, "linear_backward_workspace_bytes: null pointer");
+  if (int rc = check_linear("linear_backward_workspace_bytes", rows, inner, outer, I8M_BF16, activation, format)) return rc;
+  *bytes = BackwardPieces(nullptr, dy, x, weight, rows, inner, outer, activation, format, dx, dweight, dbias).bytes;
+  return 0;
+}
+extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_codes, const void* x_exponents, const void* weight,
+                                   const void* z, const void* z_codes, const void* z_exponents, int format, int activation,
+                                   void* dx, void* dweight, void* dbias, int rows, int inner, int outer, int dtype,
+                                   void* workspace, size_t workspace_bytes, uint32_t* status, i8m_stream_t stream) {
+  if (!dy || !status || (!dx && !dweight && !dbias)) return fail(I8M_E_ARGUMENT, "linear_backward: null pointer");
+  if (int rc = check_linear("linear_backward", rows, inner, outer, dtype, activation, format)) return rc;
+  if (dx && !weight) return fail(I8M_E_ARGUMENT, "linear_backward: dx needs the weight");
+  if (dweight && (format < 0 ? !x : !x_codes || !x_exponents))
+    return fail(I8M_E_ARGUMENT, "linear_backward: the weight's gradient needs x or its codes");
+  if (activation != ACT_NONE && (format < 0 ? !z : !z_codes || !z_exponents))
+    return fail(I8M_E_ARGUMENT, "linear_backward: an activation needs z or its codes");
+  if ((reinterpret_cast<uintptr_t>(z) | (format >= 0 ? reinterpret_cast<uintptr_t>(z_codes) : 0)) & 15u)
+    return fail(I8M_E_ARGUMENT, "linear_backward: z or its codes are not 16-byte aligned");
+  const BackwardPieces pieces(workspace, dy, x, weight, rows, inner, outer, activation, format, dx, dweight, dbias);
+  if (pieces.bytes && (!workspace || workspace_bytes < pieces.bytes))
+    return fail(I8M_E_WORKSPACE, "linear_backward: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, pieces.bytes);
+  const int inner_pitch = pad_to(inner, 8), outer_pitch = pad_to(outer, 8);
+
+  if (pieces.dz || dbias) {
+    LinearDz d{};
+    d.dy = dy; d.z = z; d.codes = z_codes; d.exponents = z_exponents;
+    d.format = format; d.activation = activation; d.dtype = dtype; d.rows = rows; d.width = outer; d.z_pitch = outer_pitch;
+    d.dz = pieces.dz; d.dz_pitch = outer_pitch; d.db = dbias; d.partials = pieces.partials;
+    if (int rc = linear_dz(d, S(stream))) return rc;
+  }
+  const void* dz = pieces.dz ? pieces.dz : dy;
+  LinearArgs a{};
+  if (dx) {
+    if (pieces.w) { if (int rc = pitch_rows(weight, pieces.w, dtype, outer, inner, inner_pitch, S(stream))) return rc; }
+    a.y = dx;
+    if (int rc = product_of(dtype, Operand{dz, outer_pitch, 0}, Operand{pieces.w ? pieces.w : weight, inner_pitch, 1}, rows, inner,
+                            outer, a, status, S(stream), "linear_dx")) return rc;
+  }
+  if (dweight) {
+    if (format >= 0) {
+      if (int rc = eight_restore(x_codes, x_exponents, rows, inner, format, pieces.x, dtype, inner_pitch, S(stream))) return rc;
+    } else if (pieces.x) {
+      if (int rc = pitch_rows(x, pieces.x, dtype, rows, inner, inner_pitch, S(stream))) return rc;
+    }
+    a.y = dweight;
+    if (int rc = product_of(dtype, Operand{dz, outer_pitch, 1}, Operand{pieces.x ? pieces.x : x, inner_pitch, 1}, outer, inner, rows,
+                            a, status, S(stream), "linear_dweight")) return rc;
+  }
+  return 0;
+}

@@ -1,0 +1,145 @@
+// Epilogue of a linear layer's products (FP16 / BF16 operands, FP32 accumulation):
+//   z = acc + bias,  y = act(z) + residual
+// in FP32, rounded once.  In training the pre-activation z leaves beside y for the backward pass, rounded to the operand
+// type or in eight bits: a thread holds 32 columns of one row, which is a group of that format, so its exponent needs no
+// exchange.  The two backward products run through the same epilogue with nothing but y.
+#pragma once
+#include "activations.cuh"
+#include "eight_bit.cuh"
+
+namespace i8m {
+
+struct LinearArgs {
+  void* y;                 // (lm, ln) in E
+  const void* bias;        // [ln] or NULL
+  const void* residual;    // (lm, ln) or NULL
+  void* z;                 // kept pre-activation: (lm, z_pitch) in E, z_pitch a multiple of 8, or NULL
+  uint8_t* codes;          // or in eight bits: (lm, 32 groups), (lm, groups), or NULL
+  uint8_t* exponents;
+  int z_pitch, groups, format, activation;
+};
+
+__device__ __forceinline__ bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Block of 16-bit values whose rows start anywhere into the patch: one element per lane, a row per request.
+__device__ __forceinline__ void load_block_elements16(const WarpPatch& wp, const uint16_t* src, size_t pitch, int rows, int cols) {
+  const uint32_t within = uint32_t((wp.lane & 7) * 2);
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    const uint16_t v = r < rows && wp.lane < cols ? src[size_t(r) * pitch + wp.lane] : uint16_t(0);
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(wp.piece(r, wp.lane >> 3) + within), "h"(v) : "memory");
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&p)[16]) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k) p[k] = pack2<E>(v[2 * k], v[2 * k + 1]);
+}
+
+// Eight bits of one group held by one thread, stored as two 16-byte vectors and a byte.
+template <int FORMAT>
+__device__ __forceinline__ void store_group(const float (&z)[32], uint8_t* codes, uint8_t* exponent) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(z[j]) & 0x7fffffffu);
+  const uint32_t byte = eight_exponent<FORMAT>(top);
+  const float inverse = eight_inverse(byte);
+  uint32_t c[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = eight_encode4<FORMAT>(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3], inverse);
+  reinterpret_cast<uint4*>(codes)[0] = make_uint4(c[0], c[1], c[2], c[3]);
+  reinterpret_cast<uint4*>(codes)[1] = make_uint4(c[4], c[5], c[6], c[7]);
+  *exponent = uint8_t(byte);
+}
+
+template <typename E>
+struct EpiLinear {
+  static constexpr int KIND = KIND_F16;
+  using Elem = E;
+  static constexpr int PARTS = 1;
+  static constexpr bool BLOCKQ = false;
+  static constexpr int PROMOTE_KB = 0;
+  static constexpr uint32_t FMT = std::is_same<E, __nv_bfloat16>::value ? 1u : 0u;
+  static constexpr uint32_t IDESC = make_idesc(1u, FMT, FMT, TILE, TILE);
+  using Args = LinearArgs;
+
+  template <class Acc>
+  static __device__ __forceinline__ void run(const GemmGeom& g, const Args& a, const TileCtx& t, const Acc& acc) {
+    const WarpPatch wp{smem_u32(t.wsm), t.lane};
+    const int wrow0 = t.row0 + 32 * t.q;
+    const bool vectors = (g.ln & 7) == 0;      // rows of y and of the residual start on 16 bytes with their tensors
+#pragma unroll 1
+    for (int c = t.c_begin; c < t.c_end; ++c) {
+      uint32_t v[32];
+      acc.load(c, v);
+      const int colb = t.col0 + c * 32;
+      if (colb >= g.ln || wrow0 >= g.lm) continue;               // uniform over the warp
+      const BlockClip clip{g.lm - wrow0, g.ln - colb};
+      float z[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
+      if (a.bias != nullptr) {
+        const E* bias = static_cast<const E*>(a.bias) + colb;
+        if (clip.cols >= 32 && on_16_bytes(bias)) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(bias) + q);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = unpack2<E>(words[k]);
+              z[8 * q + 2 * k] += f.x; z[8 * q + 2 * k + 1] += f.y;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < clip.cols) z[j] += widen<E>(bias[j]);
+        }
+      }
+      uint32_t p[16];
+      if (a.z != nullptr) {
+        pack_row<E>(z, p);
+        wp.write_own_row(p);
+        __syncwarp();
+        store_block_rows(wp, reinterpret_cast<uint8_t*>(static_cast<E*>(a.z) + size_t(wrow0) * a.z_pitch + colb),
+                         size_t(a.z_pitch) * 2, clip.rows, (a.z_pitch - colb) * 2);
+        __syncwarp();
+      }
+      if (a.codes != nullptr && t.row < g.lm) {
+        const size_t group = size_t(t.row) * a.groups + (colb >> 5);
+        if (a.format == EIGHT_INT8) store_group<EIGHT_INT8>(z, a.codes + group * 32, a.exponents + group);
+        else store_group<EIGHT_E4M3>(z, a.codes + group * 32, a.exponents + group);
+      }
+      __syncwarp();
+      with_activation(a.activation, [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = activate<decltype(act)::value>(z[j]);
+      });
+      const size_t first = size_t(wrow0) * g.ln + colb;
+      if (a.residual != nullptr) {
+        const E* r = static_cast<const E*>(a.residual) + first;
+        if (vectors && on_16_bytes(a.residual)) load_block_rows(wp, reinterpret_cast<const uint8_t*>(r), size_t(g.ln) * 2, clip.rows, clip.cols * 2);
+        else load_block_elements16(wp, reinterpret_cast<const uint16_t*>(r), size_t(g.ln), clip.rows, clip.cols);
+        __syncwarp();
+        wp.read_own_row(p);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 f = unpack2<E>(p[k]);
+          z[2 * k] += f.x; z[2 * k + 1] += f.y;
+        }
+      }
+      pack_row<E>(z, p);
+      wp.write_own_row(p);
+      __syncwarp();
+      E* y = static_cast<E*>(a.y) + first;
+      if (vectors && on_16_bytes(a.y)) store_block_rows(wp, reinterpret_cast<uint8_t*>(y), size_t(g.ln) * 2, clip.rows, clip.cols * 2);
+      else store_block_elements16(wp, reinterpret_cast<uint16_t*>(y), size_t(g.ln), clip.rows, clip.cols);
+      __syncwarp();                            // the patch is free for the next chunk
+    }
+  }
+};
+
+}  // namespace i8m

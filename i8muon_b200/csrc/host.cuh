@@ -82,7 +82,9 @@ inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // 3-D map over a row-major operand.  K-major: (batch, extent, k), box {128 bytes of K, 128 rows, 1}; MN-major:
 // (batch, k, extent), box {128 bytes along the extent, one K block of rows, 1}.  What lies beyond the tensor reads as zero.
-int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn = 0);
+// Rows may lie `pitch` elements apart (0: contiguous), and a K-major box may have fewer than 128 rows.
+int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn = 0, int pitch = 0,
+                     int box_rows = 128);
 int sm_count();   // of the current device, capped by i8m_set_cta_limit
 
 inline bool float_dtype_ok(int d) { return d == I8M_F32 || d == I8M_F16 || d == I8M_BF16; }

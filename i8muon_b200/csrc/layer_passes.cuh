@@ -1,5 +1,6 @@
 // Memory-bound passes of the layers around the stepped matrices: activations to and from eight bits, layer norm.
 #pragma once
+#include "activations.cuh"
 #include "eight_bit.cuh"
 
 namespace i8m {
@@ -193,6 +194,62 @@ column_fold_kernel(const float* __restrict__ partials, E* __restrict__ out0, E* 
     for (int i = 0; i < COLUMN_LANES; ++i) s += sh[l][i][c];
     out[col] = round_to<E>(s);
   }
+}
+
+// ====================================================================== linear layer
+// Rows copied to a pitch that tensor copies can address (a multiple of 16 bytes).
+template <typename E>
+__global__ void __launch_bounds__(256)
+pitch_rows_kernel(const E* __restrict__ src, E* __restrict__ dst, long long rows, int width, int pitch) {
+  pdl_wait();
+  const int octets = pitch / 8;
+  const long long total = rows * octets;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / octets;
+    const int col = int(i - row * octets) * 8;
+    alignas(16) E v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = col + j < width ? src[row * width + col + j] : round_to<E>(0.f);
+    *reinterpret_cast<uint4*>(dst + row * pitch + col) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+
+// What the backward pass knows of the pre-activation.
+template <typename E>
+struct PreActivation {
+  const E* z;               // (rows, z_pitch)
+  const uint8_t* codes;     // or eight bits
+  const uint8_t* exponents;
+  int z_pitch, groups;
+};
+// dz = dy act'(z) (dz may be NULL) and, where partials is not NULL, its sums over bands of rows for the bias's gradient.
+template <typename E, int FORMAT>
+__global__ void __launch_bounds__(32 * COLUMN_LANES)
+linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict__ dz, float* __restrict__ partials, long long rows,
+                 int width, int dz_pitch, long long band, int activation) {
+  pdl_wait();
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+  const long long first = blockIdx.y * band, last = first + band < rows ? first + band : rows;
+  float sum = 0.f;
+  if (col < width) {
+    with_activation(activation, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      for (long long row = first + (threadIdx.x >> 5); row < last; row += COLUMN_LANES) {
+        float v = widen<E>(dy[row * width + col]);
+        if constexpr (ACT != ACT_NONE) {
+          float z;
+          if constexpr (FORMAT >= 0)
+            z = eight_decode1<FORMAT>(kept.codes[row * kept.groups * EIGHT_GROUP + col],
+                                      eight_step(kept.exponents[row * kept.groups + col / EIGHT_GROUP]));
+          else z = widen<E>(kept.z[row * kept.z_pitch + col]);
+          v *= derivative<ACT>(z);
+        }
+        sum += v;
+        if (dz != nullptr) dz[row * dz_pitch + col] = round_to<E>(v);
+      }
+    });
+  }
+  if (partials != nullptr) store_column_sums(sum, 0.f, partials, width);
 }
 
 }  // namespace i8m

@@ -18,4 +18,21 @@ int eight_quant(const void* x, int dtype, long long rows, int width, int format,
 int eight_restore(const void* codes, const void* exponents, long long rows, int width, int format, void* out, int dtype, int pitch,
                   cudaStream_t stream);
 
+// rows of `width` 16-bit elements copied to rows of `pitch`
+int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width, int pitch, cudaStream_t stream);
+// dz = dy act'(z) into rows of dz_pitch (dz may be NULL), and db (may be NULL; partials: row_bands(rows) x 2 x width floats)
+struct LinearDz {
+  const void* dy;
+  const void* z;
+  const void *codes, *exponents;
+  int format, activation, dtype;
+  long long rows;
+  int width, z_pitch;
+  void* dz;
+  int dz_pitch;
+  void* db;
+  float* partials;
+};
+int linear_dz(const LinearDz& d, cudaStream_t stream);
+
 }  // namespace i8m

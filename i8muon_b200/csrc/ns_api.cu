@@ -62,19 +62,20 @@ int load_encode() {
 }
 }  // namespace
 
-int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn) {
+int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn, int pitch, int box_rows) {
   const int inner = mn ? extent : k, rows = mn ? k : extent;
+  if (pitch == 0) pitch = inner;
   if (int rc = load_encode()) return rc;
   if ((reinterpret_cast<uintptr_t>(ptr) & 15u) != 0)
     return fail(I8M_E_ARGUMENT, "GEMM operand is not 16-byte aligned");
-  if ((size_t(inner) * esize) % 16 != 0)
-    return fail(I8M_E_ARGUMENT, "GEMM operand row pitch (%d x %d bytes) is not a multiple of 16", inner, esize);
+  if ((size_t(pitch) * esize) % 16 != 0)
+    return fail(I8M_E_ARGUMENT, "GEMM operand row pitch (%d x %d bytes) is not a multiple of 16", pitch, esize);
   CUtensorMapDataType dt = esize == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                          : esize == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
                                       : CU_TENSOR_MAP_DATA_TYPE_UINT32;
   cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(batch)};
-  cuuint64_t strides[2] = {cuuint64_t(inner) * esize, cuuint64_t(inner) * esize * rows};
-  cuuint32_t box[3] = {cuuint32_t(128 / esize), cuuint32_t(mn ? 128 / esize : 128), 1u};
+  cuuint64_t strides[2] = {cuuint64_t(pitch) * esize, cuuint64_t(pitch) * esize * rows};
+  cuuint32_t box[3] = {cuuint32_t(128 / esize), cuuint32_t(mn ? 128 / esize : box_rows), 1u};
   cuuint32_t estr[3] = {1u, 1u, 1u};
   CUresult r = g_encode(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

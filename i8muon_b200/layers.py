@@ -1,9 +1,9 @@
 """The layers around the matrices that Muon steps: what makes their gradients.
 
-``layer_norm``, and activations kept in eight bits for the backward pass (``quantise_activation``, ``restore_activation``,
+``linear`` (bias, activation and residual in the product's epilogue), ``layer_norm``, and activations kept in eight bits for the backward pass (``quantise_activation``, ``restore_activation``,
 and the ``checkpoint=`` argument of the layers).  The functions take and return torch tensors, work on
-the current stream of the tensors' device without synchronising, and are differentiable once.  Each is one call into the
-sm_100a library forward and one backward; there is no fallback.  The reference starts at the gradient and has no counterpart.
+the current stream of the tensors' device without synchronising, and are differentiable once.  They run the sm_100a library's
+kernels; there is no fallback.  The reference starts at the gradient and has no counterpart.
 
 Eight-bit format: groups of 32 consecutive elements of a row share a power of two, the smallest 2^e with
 max|x| <= M 2^e (M = 127 for ``"int8"``, 448 for ``"fp8"``, E4M3; e >= -127), and each element is rounded to the nearest
@@ -20,13 +20,14 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import native
-from .engine import on_device, raw_stream
+from .engine import on_device, raw_stream, status_word
 
-__all__ = ["layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]
+__all__ = ["linear", "layer_norm", "quantise_activation", "restore_activation", "QuantisedActivation"]
 
 GROUP = 32
 _FORMATS = {None: native.EIGHT_NONE, "int8": native.EIGHT_INT8, "fp8": native.EIGHT_E4M3}
 _CODE_TYPES = {native.EIGHT_INT8: torch.int8, native.EIGHT_E4M3: torch.float8_e4m3fn}
+_ACTIVATIONS = {None: 0, "relu": 1, "relu2": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -211,3 +212,106 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
         return _LayerNorm.apply(x, weight, bias, eps, fmt)
     return _norm_forward(x.detach().contiguous(), None if weight is None else weight.contiguous(),
                          None if bias is None else bias.contiguous(), eps, native.EIGHT_NONE, False)[0]
+
+
+# ---------------------------------------------------------------------- linear
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
+def _linear_forward(x, weight, bias, residual, activation, fmt, keep):
+    """(y, z, codes of z, their exponents) of contiguous tensors; the last three are None where nothing is kept."""
+    inner, outer = x.shape[-1], weight.shape[0]
+    rows, device = x.numel() // inner, x.device
+    with on_device(device.index):
+        y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
+        z = codes = exponents = None
+        if keep:
+            if fmt == native.EIGHT_NONE:
+                z = torch.empty((rows, -(-outer // 8) * 8), dtype=x.dtype, device=device)
+            else:
+                codes, exponents = _empty_codes((rows,), outer, device)
+        if rows:
+            size = 0
+            if inner % 8 or (x.data_ptr() | weight.data_ptr()) % 16:
+                size = native.linear_workspace_bytes(x.data_ptr(), weight.data_ptr(), rows, inner, outer)
+            workspace = _workspace(size, device)
+            native.call("i8m_linear", x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z),
+                        _ptr(codes), _ptr(exponents), fmt, activation, rows, inner, outer, native.torch_dtype_code(x.dtype),
+                        _ptr(workspace), size, status_word(device).data_ptr(), raw_stream(device.index))
+    return y, z, codes, exponents
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, fmt):
+        x, weight = x.contiguous(), weight.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        residual = None if residual is None else residual.contiguous()
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        keep_z = activation != 0 and (need_x or need_w or need_b)
+        y, z, z_codes, z_exponents = _linear_forward(x, weight, bias, residual, activation, fmt, keep_z)
+        x_codes = x_exponents = None
+        if need_w and fmt != native.EIGHT_NONE:
+            with on_device(x.device.index):
+                x_codes, x_exponents = _quantise(x, x.numel() // x.shape[-1], x.shape[-1], fmt, (x.numel() // x.shape[-1],))
+        ctx.activation, ctx.fmt, ctx.x_shape, ctx.w_shape, ctx.dtype = activation, fmt, x.shape, weight.shape, x.dtype
+        ctx.save_for_backward(x if need_w and fmt == native.EIGHT_NONE else None, x_codes, x_exponents,
+                              weight if need_x else None, z, z_codes, z_exponents)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, x_codes, x_exponents, weight, z, z_codes, z_exponents = ctx.saved_tensors
+        outer, inner = ctx.w_shape
+        rows, device = dy.numel() // outer, dy.device
+        dresidual = dy if ctx.needs_input_grad[3] else None
+        dx = dw = db = None
+        if any(ctx.needs_input_grad[:3]):
+            dy = dy.contiguous()
+            with on_device(device.index):
+                make = torch.zeros if rows == 0 else torch.empty
+                dx, dw, db = (make(shape, dtype=ctx.dtype, device=device) if wanted else None
+                              for wanted, shape in zip(ctx.needs_input_grad, (ctx.x_shape, ctx.w_shape, (outer,))))
+                if rows:
+                    wants = int(dx is not None), int(dw is not None), int(db is not None)
+                    size = native.linear_backward_workspace_bytes(dy.data_ptr(), _ptr(x), _ptr(weight), rows, inner, outer,
+                                                                  ctx.activation, ctx.fmt, *wants)
+                    workspace = _workspace(size, device)
+                    native.call("i8m_linear_backward", dy.data_ptr(), _ptr(x), _ptr(x_codes), _ptr(x_exponents), _ptr(weight), _ptr(z),
+                                _ptr(z_codes), _ptr(z_exponents), ctx.fmt, ctx.activation, _ptr(dx), _ptr(dw), _ptr(db), rows,
+                                inner, outer, native.torch_dtype_code(ctx.dtype), _ptr(workspace), size,
+                                status_word(device).data_ptr(), raw_stream(device.index))
+        return dx, dw, db, dresidual, None, None
+
+
+def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activation: Optional[str] = None,
+           residual: Optional[Tensor] = None, checkpoint: Optional[str] = None) -> Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one product.
+
+    ``x`` (..., inner) in float16 or bfloat16, ``weight`` (outer, inner) as ``torch.nn.Linear`` holds it, ``bias`` (outer),
+    ``residual`` (..., outer), all of one type.  ``activation``: None, "relu", "relu2" (max(z, 0)^2), "gelu" (with the
+    error function), "gelu_tanh" or "silu".  Sums, bias, activation and residual are FP32; the result is rounded once.
+
+    For the backward pass ``x`` and, with an activation, the pre-activation rounded to the type of ``x`` are kept, or both in
+    eight bits with ``checkpoint="int8"`` or ``"fp8"``.  The gradients are those of the formula at what was kept; the
+    gradient of the pre-activation is rounded to the type of ``x`` once, as the operand of the two backward products.
+
+    A device-side wait that runs out is reported through the status word that ``check_status()`` and ``Muon.step()`` read."""
+    fmt = _format(checkpoint, "linear")
+    if activation is not None and not isinstance(activation, str) or activation not in _ACTIVATIONS:
+        raise ValueError("linear: activation must be None, 'relu', 'relu2', 'gelu', 'gelu_tanh' or 'silu'")
+    rows, inner = _check_rows("linear", x, (torch.float16, torch.bfloat16))
+    if not isinstance(weight, Tensor) or weight.ndim != 2 or weight.shape[1] != inner or weight.dtype != x.dtype or weight.shape[0] < 1:
+        raise ValueError(f"linear: weight must be a matrix of {inner} columns of the input's type")
+    outer = weight.shape[0]
+    _check_vector("linear", "bias", bias, outer, x.dtype)
+    if residual is not None and (not isinstance(residual, Tensor) or residual.shape != (*x.shape[:-1], outer)
+                                 or residual.dtype != x.dtype):
+        raise ValueError("linear: residual must have the shape and type of the result")
+    _check_device("linear", x, weight, bias, residual)
+    if _any_gradient(x, weight, bias, residual):
+        return _Linear.apply(x, weight, bias, residual, _ACTIVATIONS[activation], fmt)
+    return _linear_forward(x.detach().contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
+                           None if residual is None else residual.contiguous(), _ACTIVATIONS[activation], native.EIGHT_NONE, False)[0]

@@ -84,6 +84,12 @@ _SIGNATURES = {
     "i8m_layer_norm_scratch_bytes": (c_int, [c_longlong, c_int, POINTER(c_size_t)]),
     "i8m_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, c_int, _P, c_size_t,
                                         _P]),
+    "i8m_linear_workspace_bytes": (c_int, [_P, _P, c_int, c_int, c_int, POINTER(c_size_t)]),
+    "i8m_linear": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
+    "i8m_linear_backward_workspace_bytes": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                                    POINTER(c_size_t)]),
+    "i8m_linear_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, _P,
+                                    c_size_t, _P, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -155,6 +161,19 @@ def stats_scratch_bytes(batch, count) -> int:
 def layer_norm_scratch_bytes(rows, width) -> int:
     size = c_size_t(0)
     call("i8m_layer_norm_scratch_bytes", rows, width, ctypes.byref(size))
+    return size.value
+
+
+def linear_workspace_bytes(x, weight, rows, inner, outer) -> int:
+    size = c_size_t(0)
+    call("i8m_linear_workspace_bytes", x, weight, rows, inner, outer, ctypes.byref(size))
+    return size.value
+
+
+def linear_backward_workspace_bytes(dy, x, weight, rows, inner, outer, activation, fmt, dx, dweight, dbias) -> int:
+    size = c_size_t(0)
+    call("i8m_linear_backward_workspace_bytes", dy, x, weight, rows, inner, outer, activation, fmt, dx, dweight, dbias,
+         ctypes.byref(size))
     return size.value
 
 

@@ -302,6 +302,33 @@ int i8m_layer_norm_backward(const void* dy_device, const void* x_device, const f
                             void* dx_device, void* dweight_device, void* dbias_device, long long rows, int width, int dtype,
                             void* scratch_device, size_t scratch_bytes, i8m_stream_t stream);
 
+/* Linear layer: z = x weight^T + bias, y = act(z) + residual, sums in FP32, y rounded once to `dtype` (I8M_F16 or I8M_BF16:
+ * the type of every tensor here).  x (rows, inner), weight (outer, inner), bias [outer] or NULL, residual (rows, outer) or
+ * NULL, y (rows, outer), all contiguous.
+ * For the backward pass of an activation the product also writes the pre-activation: z (rows, outer rounded up to 8) where
+ * `format` is I8M_EIGHT_NONE, z_codes and z_exponents otherwise (16-byte aligned; NULL: not kept).
+ * workspace (16-byte aligned): copies of x or weight whose rows do not start on multiples of 16 bytes; often 0 bytes. */
+enum i8m_activation {
+  I8M_ACT_NONE = 0, I8M_ACT_RELU = 1, I8M_ACT_RELU2 = 2 /* max(z, 0)^2 */, I8M_ACT_GELU = 3 /* z Phi(z) */,
+  I8M_ACT_GELU_TANH = 4, I8M_ACT_SILU = 5
+};
+int i8m_linear_workspace_bytes(const void* x_device, const void* weight_device, int rows, int inner, int outer, size_t* bytes);
+int i8m_linear(const void* x_device, const void* weight_device, const void* bias_device, const void* residual_device,
+               void* y_device, void* z_device, void* z_codes_device, void* z_exponents_device, int format, int activation,
+               int rows, int inner, int outer, int dtype, void* workspace_device, size_t workspace_bytes,
+               uint32_t* status_device, i8m_stream_t stream);
+/* Gradients of the above (the residual's is dy itself); dx, dweight, dbias may each be NULL.  dz = dy act'(z) at the kept z,
+ * rounded to `dtype` as the operand of dx = dz weight and dweight = dz^T x; dbias sums the unrounded dz over bands of rows in
+ * a fixed order.  x, or its codes (i8m_activation_quant) where `format` names a format, serves dweight; z or its codes serve an
+ * activation.  dx, dweight and dbias in the arguments of the query are truth values. */
+int i8m_linear_backward_workspace_bytes(const void* dy_device, const void* x_device, const void* weight_device, int rows, int inner,
+                                        int outer, int activation, int format, int dx, int dweight, int dbias, size_t* bytes);
+int i8m_linear_backward(const void* dy_device, const void* x_device, const void* x_codes_device, const void* x_exponents_device,
+                        const void* weight_device, const void* z_device, const void* z_codes_device,
+                        const void* z_exponents_device, int format, int activation, void* dx_device, void* dweight_device,
+                        void* dbias_device, int rows, int inner, int outer, int dtype, void* workspace_device,
+                        size_t workspace_bytes, uint32_t* status_device, i8m_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

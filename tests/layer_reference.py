@@ -109,6 +109,92 @@ def layer_norm_gradients(dy, u, tol_u, rstd, rel_rstd, w, dtype):
             (("dx", raw, tol), ("dw", dw, tol_dw), ("db", db, tol_db))}
 
 
+# ---------------------------------------------------------------------- linear
+def activation(z, name):
+    """The activation, its derivative and (a bound on) the slope of that."""
+    zero, one = torch.zeros_like(z), torch.ones_like(z)
+    if name is None:
+        return z, one, zero
+    if name == "relu":
+        return z.clamp_min(0), (z > 0).double(), zero
+    if name == "relu2":
+        return z.clamp_min(0).square(), 2 * z.clamp_min(0), 2 * one
+    if name == "silu":
+        s = torch.sigmoid(z)
+        ds = s * (1 - s)
+        return z * s, s + z * ds, 2 * ds + z * ds * (1 - 2 * s)
+    if name == "gelu":
+        cdf, pdf = torch.special.ndtr(z), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return z * cdf, cdf + z * pdf, pdf * (2 - z * z)
+    c, k = math.sqrt(2 / math.pi), 0.044715
+    u, du, ddu = c * (z + k * z ** 3), c * (1 + 3 * k * z * z), 6 * c * k * z
+    t = torch.tanh(u)
+    dt = (1 - t * t) * du
+    return z * (1 + t) / 2, (1 + t) / 2 + z * dt / 2, dt + z / 2 * ((1 - t * t) * ddu - 2 * t * dt * du)
+
+
+def activation_slack(z, name):
+    """What evaluating an activation and its derivative in FP32 may lose: a few roundings, an exponential whose argument is
+    no larger than 1 + z^2 and rounded relative to itself, a quotient, and a published approximation's last places - 32
+    roundings per unit of the argument, of the terms that are added up."""
+    y, d1, _ = activation(z, name)
+    if name is None:
+        return torch.zeros_like(z), torch.zeros_like(z)
+    gate = torch.where(z == 0, torch.full_like(z, 0.5), y / z)
+    unit = 32 * EPS * (1 + z * z)
+    return unit * y.abs(), unit * (gate.abs() + d1.abs())
+
+
+def product_slack(a, b):
+    """What a product a b^T with FP32 accumulation of 16 terms at a time may lose: each instruction's sum is truncated,
+    two units in the last place of at most the sum of magnitudes; splitting the sum adds a few roundings."""
+    return (a.shape[1] / 16 + 24) * 4 * EPS * (a.abs() @ b.abs().t())
+
+
+def linear(x, w, b, r, name, dtype):
+    """(y, tolerance, z, tolerance of z)."""
+    z = x @ w.t() + (0 if b is None else b)
+    tol_z = product_slack(x, w) + 2 * EPS * z.abs()
+    y, d1, _ = activation(z, name)
+    # the derivatives are bounded over the interval by their values and the next derivative's change
+    slope = d1.abs() + 3 * tol_z
+    if name == "relu":
+        slope = torch.ones_like(z)
+    tol = tol_z * slope + activation_slack(z, name)[0]
+    if r is not None:
+        tol = tol + 2 * EPS * (y.abs() + r.abs())
+        y = y + r
+    return y, tol + half_step(y.abs() + tol, dtype), z, tol_z
+
+
+def rounded_with_slack(z, slack, dtype):
+    """z rounded to a type, and how far the rounding of values up to ``slack`` away may be from that."""
+    v = z.to(dtype).double()
+    return v, torch.maximum((z + slack).to(dtype).double() - v, v - (z - slack).to(dtype).double())
+
+
+def linear_gradients(dy, x, w, kept_z, off_z, name, dtype):
+    """{name: (gradient, tolerance)} at the kept rows x and a kept pre-activation known to ``off_z``."""
+    _, d1, d2 = activation(kept_z, name)
+    dz = dy * d1
+    if name is None:
+        off = torch.zeros_like(dz)
+        exact = dz
+    else:
+        # relu's derivative may differ where z is on either side of zero
+        flip = ((kept_z.abs() <= off_z) & (off_z > 0)).double() if name == "relu" else 0
+        off = dy.abs() * (activation_slack(kept_z, name)[1] + off_z * (d2.abs() + 3 * off_z) + flip)
+        exact = dz
+        off_rounded = off + half_step(dz.abs() + off, dtype)
+    rounded = off if name is None else off_rounded
+    dx, dw, db = exact @ w, exact.t() @ x, exact.sum(0)
+    tol_dx = rounded @ w.abs() + product_slack(exact.abs() + rounded, w.t())
+    tol_dw = rounded.t() @ x.abs() + product_slack((exact.abs() + rounded).t(), x.t())
+    tol_db = off.sum(0) + (row_chain(dy.shape[0]) + 3) * EPS * exact.abs().sum(0)
+    return {key: (v, t + half_step(v.abs() + t, dtype)) for key, v, t in
+            (("dx", dx, tol_dx), ("dw", dw, tol_dw), ("db", db, tol_db))}
+
+
 def assert_within(got, want, tol, what):
     got = got.double()
     off = (got - want).abs()

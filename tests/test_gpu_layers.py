@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import layer_reference as ref
-from i8muon_b200 import layer_norm, quantise_activation, restore_activation
+from i8muon_b200 import check_status, layer_norm, linear, quantise_activation, restore_activation
 
 pytestmark = pytest.mark.gpu
 TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -208,3 +208,147 @@ def test_layer_norm_edges(cuda_device):
     dx, = torch.autograd.grad(layer_norm(x, w).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+# ---------------------------------------------------------------------- linear
+ACTS = (None, "relu", "relu2", "gelu", "gelu_tanh", "silu")
+
+
+def linear_inputs(rows, inner, outer, dtype, device, bias=True, residual=True, seed=0):
+    x = normal((rows, inner), seed + 1, dtype, device)
+    w = normal((outer, inner), seed + 2, dtype, device, inner ** -0.5)
+    b = normal((outer,), seed + 3, dtype, device, 0.3) if bias else None
+    r = normal((rows, outer), seed + 4, dtype, device) if residual else None
+    return x, w, b, r, normal((rows, outer), seed + 5, dtype, device)
+
+
+def check_linear(x, w, b, r, dy, act, checkpoint=None):
+    dtype = x.dtype
+    leaves = {name: t.detach().requires_grad_() for name, t in (("x", x), ("w", w), ("b", b), ("r", r)) if t is not None}
+    y = linear(leaves["x"], leaves["w"], leaves.get("b"), activation=act, residual=leaves.get("r"), checkpoint=checkpoint)
+    got = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    assert torch.equal(linear(x, w, b, activation=act, residual=r), y)      # the same values where nothing is kept
+    check_status()
+    want, tol, z, tol_z = ref.linear(double(x), double(w), double(b), double(r), act, dtype)
+    ref.assert_within(y, want, tol, "y")
+    if checkpoint is None:
+        kept, off = ref.rounded_with_slack(z, tol_z, dtype)
+        kept_x = double(x)
+    else:
+        kept, off = ref.kept_with_slack(z, tol_z, checkpoint)
+        kept_x = ref.kept(double(x), checkpoint)
+    wants = ref.linear_gradients(double(dy), kept_x, double(w), kept, off, act, dtype)
+    for name in ("x", "w", "b"):
+        if name in got:
+            assert got[name].dtype == dtype
+            ref.assert_within(got[name], *wants["d" + name], "d" + name)
+    if r is not None:
+        assert torch.equal(got["r"], dy)
+
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 8, 8), (2, 7, 5), (1, 64, 128), (3, 4096, 64), (16, 1000, 200), (17, 72, 1001), (33, 129, 130), (64, 256, 512),
+                 (65, 513, 384), (128, 128, 128), (129, 264, 257), (200, 1001, 333), (257, 768, 640), (1000, 96, 1000), (2050, 320, 72)]
+
+
+@pytest.mark.parametrize("shape", LINEAR_SHAPES)
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("act", ACTS)
+def test_linear_and_its_gradients(cuda_device, shape, dtype, act):
+    extras = sum(shape) % 4
+    check_linear(*linear_inputs(*shape, dtype, cuda_device, bias=extras != 1, residual=extras >= 2), act)
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 1), (2, 33, 5), (16, 1000, 200), (65, 96, 384), (130, 264, 257), (300, 768, 640)])
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("checkpoint", FORMATS)
+def test_linear_gradients_at_what_was_kept_in_eight_bits(cuda_device, shape, dtype, act, checkpoint):
+    check_linear(*linear_inputs(*shape, dtype, cuda_device), act, checkpoint)
+
+
+@pytest.mark.parametrize("shape", [(4096, 512, 1024), (300, 8192, 256), (12000, 256, 256), (2, 2048, 9000)])
+def test_linear_over_many_tiles_and_long_sums(cuda_device, shape):
+    check_linear(*linear_inputs(*shape, torch.bfloat16, cuda_device), "gelu")
+
+
+def test_linear_takes_any_strides_and_leading_dimensions(cuda_device):
+    dtype = torch.bfloat16
+    base, wbase = normal((4, 6, 80), 1, dtype, cuda_device), normal((50, 160), 2, dtype, cuda_device, 0.1)
+    for x, w in ((base.transpose(0, 1), wbase[:, :80]), (base[..., 1:65], wbase[:, 3:67]), (base[:, ::3], wbase[:, ::2]), (base[0, 0], wbase[5:, 80:]),
+                 (base.reshape(-1)[3:3 + 640].view(10, 64), wbase.reshape(-1)[1:1 + 640].view(10, 64)),
+                 (base[0, :1].expand(5, 80), wbase[:1, :80].expand(7, 80)),
+                 (base[..., :50], wbase.t()[7:11, :])):
+        b = normal((2 * w.shape[0],), 3, dtype, cuda_device)[1::2]
+        r = normal((w.shape[0], *x.shape[:-1]), 4, dtype, cuda_device).movedim(0, -1)
+        dy = normal((w.shape[0], *x.shape[:-1]), 5, dtype, cuda_device).movedim(0, -1)
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = linear(leaves[0], leaves[1], leaves[2], activation="silu", residual=leaves[3])
+        got = torch.autograd.grad(y, leaves, dy)
+        flat = [t.reshape(-1, t.shape[-1]) for t in (x, r, dy)]
+        want, tol, z, tol_z = ref.linear(flat[0].double(), w.double(), b.double(), flat[1].double(), "silu", dtype)
+        assert y.shape == (*x.shape[:-1], w.shape[0]) and y.is_contiguous()
+        ref.assert_within(y.reshape(want.shape), want, tol, "y")
+        wants = ref.linear_gradients(flat[2].double(), flat[0].double(), w.double(), *ref.rounded_with_slack(z, tol_z, dtype), "silu", dtype)
+        for name, g, t in zip(("dx", "dw", "db"), got, leaves):
+            assert g.shape == t.shape
+            ref.assert_within(g.reshape(wants[name][0].shape), *wants[name], name)
+        assert torch.equal(got[3], dy)
+
+
+def test_linear_gradients_against_differences(cuda_device):
+    """Central differences of the formula in 64 bits with h = 1e-4: off by less than 1e-6 from the derivative, the kernels'
+    gradients by their rounding to FP16 (2^-11 each for dz and the result, values below 4) and FP32 sums."""
+    x, w, b, r, dy = linear_inputs(5, 24, 16, torch.float16, cuda_device)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    for act in ("gelu", "gelu_tanh", "silu"):
+        got = torch.autograd.grad(linear(x, w, b, activation=act, residual=r), leaves, dy)
+        args = [double(t) for t in leaves]
+        for k, t in enumerate(args):
+            for i in range(0, t.numel(), 11):
+                side = []
+                for sign in (1, -1):
+                    moved = [a.clone() for a in args]
+                    moved[k].view(-1)[i] += sign * 1e-4
+                    side.append((ref.activation(moved[0] @ moved[1].t() + moved[2], act)[0] * double(dy)).sum().item())
+                # dz's roundings add up over at most 16 products, z was kept in FP16 (2^-11 of z times the slope's change)
+                assert abs((side[0] - side[1]) / 2e-4 - got[k].reshape(-1)[i].item()) < 2.0 ** -11 * 3 * 4 * 4
+
+
+def test_linear_edges(cuda_device):
+    dtype = torch.bfloat16
+    w, b = normal((8, 16), 1, dtype, cuda_device).requires_grad_(), normal((8,), 2, dtype, cuda_device).requires_grad_()
+    # no rows
+    x = torch.zeros(0, 3, 16, dtype=dtype, device=cuda_device, requires_grad=True)
+    for checkpoint in (None, "fp8"):
+        y = linear(x, w, b, activation="gelu", checkpoint=checkpoint)
+        dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+        assert y.shape == (0, 3, 8) and dx.shape == x.shape and not dw.any() and not db.any()
+    # a vector is a row
+    x = normal((16,), 3, dtype, cuda_device).requires_grad_()
+    y = linear(x, w, b)
+    assert y.shape == (8,)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == (16,)
+    # an element that is not finite spoils its own row, and nothing else
+    x = normal((200, 16), 4, dtype, cuda_device)
+    x[130, 5] = math.nan
+    for act in ACTS:
+        y = linear(x, w, b, activation=act)
+        assert torch.isnan(y[130]).all() and torch.isfinite(y[:130]).all() and torch.isfinite(y[131:]).all()
+    # each gradient alone
+    x = normal((40, 16), 5, dtype, cuda_device).requires_grad_()
+    r = normal((40, 8), 6, dtype, cuda_device).requires_grad_()
+    dy = normal((40, 8), 7, dtype, cuda_device)
+    for checkpoint in (None, "int8"):
+        def y():
+            return linear(x, w, b, activation="silu", residual=r, checkpoint=checkpoint)
+        together = torch.autograd.grad(y(), (x, w, b, r), dy)
+        for t, g in zip((x, w, b, r), together):
+            others = [s for s in (x, w, b, r) if s is not t]
+            for s in others:
+                s.requires_grad_(False)
+            assert torch.equal(torch.autograd.grad(y(), t, dy)[0], g)
+            for s in others:
+                s.requires_grad_(True)
+    with pytest.raises(RuntimeError):
+        g, = torch.autograd.grad(linear(x, w).float().square().sum(), x, create_graph=True)
+        g.float().sum().backward()

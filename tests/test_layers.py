@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from i8muon_b200 import QuantisedActivation, layer_norm, native, quantise_activation, restore_activation
+from i8muon_b200 import QuantisedActivation, layer_norm, linear, native, quantise_activation, restore_activation
 from i8muon_b200.build import build
 
 
@@ -11,7 +11,7 @@ def library():
     build()
 
 
-X = torch.zeros(3, 40)
+X, H, W = torch.zeros(3, 40), torch.zeros(3, 40).half(), torch.zeros(8, 40).half()
 
 
 @pytest.mark.parametrize("call, message", [
@@ -32,6 +32,20 @@ X = torch.zeros(3, 40)
     (lambda: layer_norm(X, eps=float("nan")), "eps must be >= 0"),
     (lambda: layer_norm(torch.zeros(2, 0)), "must not be empty"),
     (lambda: layer_norm(X, torch.zeros(40)), "needs CUDA"),
+    (lambda: linear(X, torch.zeros(8, 40)), "float16 or bfloat16"),
+    (lambda: linear(H, torch.zeros(8, 40)), "40 columns of the input's type"),
+    (lambda: linear(H, W.t()), "40 columns"),
+    (lambda: linear(H, W[None]), "40 columns"),
+    (lambda: linear(H, W[:0]), "40 columns"),
+    (lambda: linear(H, W, torch.zeros(7).half()), "bias must be a vector of 8"),
+    (lambda: linear(H, W, torch.zeros(8)), "bias must be a vector of 8"),
+    (lambda: linear(H, W, activation="tanh"), "activation must be"),
+    (lambda: linear(H, W, activation=1), "activation must be"),
+    (lambda: linear(H, W, residual=torch.zeros(8).half()), "shape and type of the result"),
+    (lambda: linear(H, W, residual=torch.zeros(3, 8)), "shape and type of the result"),
+    (lambda: linear(H, W, checkpoint="bf16"), "checkpoint must be"),
+    (lambda: linear(torch.zeros(3, 0).half(), torch.zeros(8, 0).half()), "must not be empty"),
+    (lambda: linear(H, W), "needs CUDA"),
 ])
 def test_refusals(call, message):
     with pytest.raises(ValueError, match=message):
@@ -74,3 +88,34 @@ def test_native_argument_errors_are_codes():
     need = native.layer_norm_scratch_bytes(4, 8)
     assert need == 4 * 2 * 8 * 4
     assert backward(dw=16) == -2 and backward(dw=16, scratch=16, size=need - 1) == -2
+
+
+def test_native_linear_argument_errors_are_codes():
+    lib = native.library()
+    p = 1 << 20      # 16-byte aligned, never dereferenced: every call is refused before a launch
+
+    def forward(*, x=p, w=p, y=p, z=None, codes=None, exponents=None, fmt=-1, act=0, rows=4, inner=16, outer=8, dtype=2, ws=None,
+                size=0, status=p):
+        return lib.i8m_linear(x, w, None, None, y, z, codes, exponents, fmt, act, rows, inner, outer, dtype, ws, size, status, None)
+    for bad in (dict(x=None), dict(w=None), dict(y=None), dict(status=None), dict(rows=0), dict(inner=0), dict(outer=0),
+                dict(dtype=0), dict(act=6), dict(act=-1), dict(fmt=2), dict(fmt=0, codes=p), dict(z=p + 8), dict(fmt=0, codes=p + 4, exponents=p)):
+        assert forward(**bad) == -1, bad
+    assert forward(inner=(1 << 24) + 8) == -4
+    assert forward(rows=(1 << 31) - 1) == -4
+    assert forward(inner=17) == -2 and forward(x=p + 2) == -2
+    need = native.linear_workspace_bytes(p, p, 4, 17, 8)
+    assert need >= (4 + 8) * 24 * 2
+    assert forward(inner=17, ws=p, size=need - 1) == -2
+    assert native.linear_workspace_bytes(p, p, 4, 16, 8) == 0
+    assert native.linear_workspace_bytes(p + 2, p, 4, 16, 8) >= 4 * 16 * 2
+
+    def backward(*, dy=p, x=p, codes=None, w=p, z=None, z_codes=None, fmt=-1, act=0, dx=p, dw=None, db=None, outer=8, ws=None, size=0):
+        return lib.i8m_linear_backward(dy, x, codes, codes, w, z, z_codes, z_codes, fmt, act, dx, dw, db, 4, 16, outer, 2, ws, size, p, None)
+    for bad in (dict(dy=None), dict(dx=None), dict(w=None), dict(x=None, dw=p), dict(fmt=0, dw=p), dict(act=3), dict(act=3, fmt=0),
+                dict(act=3, z=p + 2)):
+        assert backward(**bad) == -1, bad
+    assert backward(act=3, z=p) == -2            # dz needs room
+    assert backward(outer=9) == -2               # dy's rows start anywhere: a copy
+    assert backward(dx=None, db=p) == -2         # partial sums
+    assert native.linear_backward_workspace_bytes(p, p, p, 4, 16, 8, 0, -1, 1, 1, 0) == 0
+    assert native.linear_backward_workspace_bytes(p, p, p, 4, 16, 8, 0, 0, 0, 1, 0) >= 4 * 16 * 2
