@@ -15,7 +15,8 @@ from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIBRARY = CSRC / "libi8muon_b200.so"
-SOURCES = ("ns_api.cu", "api_float.cu", "api_int8.cu", "api_bq.cu", "api_passes.cu", "api_layers.cu", "api_linear.cu")
+SOURCES = ("ns_api.cu", "api_float.cu", "api_int8.cu", "api_bq.cu", "api_passes.cu", "api_layers.cu", "api_norm.cu",
+           "api_linear.cu")
 NVCC_FLAGS = (
     "-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
     # FP32 expressions are evaluated exactly as written; fused multiply-adds

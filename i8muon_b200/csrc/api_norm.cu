@@ -1,0 +1,160 @@
+// C ABI: layer norm.
+#include "host.cuh"
+#include "layers.cuh"
+#include "layer_norm.cuh"
+
+#include <initializer_list>
+
+using namespace i8m;
+
+// ================================================================== layer norm
+namespace {
+
+int check_norm(const char* name, const void* a, const void* b, long long rows, int width, int dtype, const void* codes,
+               const void* exponents, int format) {
+  if (!a || !b) return fail(I8M_E_ARGUMENT, "%s: null pointer", name);
+  if (rows < 1 || width < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
+  if (!float_dtype_ok(dtype)) return fail(I8M_E_ARGUMENT, "%s: bad dtype %d", name, dtype);
+  if (format < -1 || format > EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
+  if (format >= 0 && (!codes || !exponents)) return fail(I8M_E_ARGUMENT, "%s: null codes or exponents", name);
+  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %d is above %d", name, width, MAX_LAYER_WIDTH);
+  if (rows > MAX_LAYER_ROWS) return fail(I8M_E_LIMIT, "%s: %lld rows are above %lld", name, rows, MAX_LAYER_ROWS);
+  return 0;
+}
+#define DISPATCH_FORMAT(format, F, ...)                                       \
+  do {                                                                        \
+    if ((format) == EIGHT_INT8) { constexpr int F = EIGHT_INT8; __VA_ARGS__; } \
+    else if ((format) == EIGHT_E4M3) { constexpr int F = EIGHT_E4M3; __VA_ARGS__; } \
+    else { constexpr int F = -1; __VA_ARGS__; }                               \
+  } while (0)
+// Calls f(kernel family) for the shape.
+template <bool W, int V>
+struct LnFamily {
+  static constexpr bool WARP = W;
+  static constexpr int OCTETS = V;
+};
+template <int MOST, class F>
+void with_ln_shape(const LnShape& s, F&& f) {
+  if (s.threads == 32 && s.octets == 1) f(LnFamily<true, 1>{});
+  else if (s.threads == 32 && s.octets == 2) f(LnFamily<true, 2>{});
+  else if (MOST == 4 && s.threads == 32) f(LnFamily<true, MOST>{});
+  else if (MOST == 2 && s.octets == 2) f(LnFamily<false, MOST>{});
+  else f(LnFamily<false, 4>{});
+}
+// Rows that start on 16 bytes throughout.
+bool ln_vectors(int width, std::initializer_list<const void*> tensors) {
+  uintptr_t bits = 0;
+  for (const void* p : tensors) bits |= reinterpret_cast<uintptr_t>(p);
+  return width % 8 == 0 && (bits & 15u) == 0;
+}
+}  // namespace
+
+extern "C" int i8m_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                              void* codes, void* exponents, int format, long long rows, int width, int dtype, float eps,
+                              i8m_stream_t stream) {
+  if (int rc = check_norm("layer_norm", x, y, rows, width, dtype, codes, exponents, format)) return rc;
+  const int groups = eight_groups(width);
+  const LnShape shape = ln_shape(width, LN_FORWARD_OCTETS);
+  uint8_t *c = static_cast<uint8_t*>(codes), *e = static_cast<uint8_t*>(exponents);
+  if (!shape.octets) {
+    const unsigned grid = unsigned(std::min<long long>(rows, 148LL * 8));
+    DISPATCH_IN(dtype, E, DISPATCH_FORMAT(format, F, (launch(
+        ln_forward_loop_kernel<E, F>, grid, LN_THREADS, 0, S(stream), static_cast<const E*>(x), static_cast<const E*>(weight),
+        static_cast<const E*>(bias), static_cast<E*>(y), mean, rstd, c, e, rows, width, groups, eps))));
+  } else {
+    const bool vectors = ln_vectors(width, {x, weight, bias, format >= 0 ? codes : nullptr}) && on_octets(y, dtype_size(dtype));
+    int rc = 0;
+    DISPATCH_IN(dtype, E, with_ln_shape<LN_FORWARD_OCTETS>(shape, [&](auto family) {
+      using Family = decltype(family);
+      constexpr int V = Family::OCTETS;
+      auto kernel = vectors ? ln_forward_kernel<E, Family::WARP, V, true> : ln_forward_kernel<E, Family::WARP, V, false>;
+      const int block = shape.block();
+      constexpr size_t STAGES = LN_STAGES<E, Family::WARP, V, 1>;
+      const size_t smem = vectors ? STAGES * block * V * 8 * sizeof(E) : 0;
+      static SmemAllowed allowed;
+      if (vectors) rc = allow_smem(allowed, kernel, STAGES * ln_stage_bytes<E, Family::WARP, V>(1));
+      if (rc) return;
+      launch(kernel, unsigned(std::min<long long>(cdiv(rows, shape.rows_of_block()), 148LL * shape.resident(512, smem))), block, smem, S(stream),
+             static_cast<const E*>(x), static_cast<const E*>(weight), static_cast<const E*>(bias), static_cast<E*>(y), mean, rstd,
+             c, e, format, rows, width, groups, eps);
+    }));
+    if (rc) return rc;
+  }
+  LAUNCH_CHECK("layer_norm");
+  return 0;
+}
+
+extern "C" int i8m_layer_norm_scratch_bytes(long long rows, int width, size_t* bytes) {
+  if (rows < 1 || width < 1 || !bytes) return fail(I8M_E_ARGUMENT, "layer_norm_scratch_bytes: bad argument");
+  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "layer_norm_scratch_bytes: width %d is above %d", width, MAX_LAYER_WIDTH);
+  *bytes = size_t(ln_bands(rows, width)) * 2 * size_t(width) * sizeof(float);
+  return 0;
+}
+extern "C" int i8m_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* codes,
+                                       const void* exponents, int format, const void* weight, void* dx, void* dweight,
+                                       void* dbias, long long rows, int width, int dtype, void* scratch, size_t scratch_bytes,
+                                       i8m_stream_t stream) {
+  if (int rc = check_norm("layer_norm_backward", dy, rstd, rows, width, dtype, codes, exponents, format)) return rc;
+  if (format < 0 && (!x || !mean)) return fail(I8M_E_ARGUMENT, "layer_norm_backward: neither x and its means nor codes");
+  if (!dx && !dweight && !dbias) return fail(I8M_E_ARGUMENT, "layer_norm_backward: nothing to compute");
+  size_t need = 0;
+  if (int rc = i8m_layer_norm_scratch_bytes(rows, width, &need)) return rc;
+  const bool sums = dweight || dbias;
+  if (sums && (!scratch || scratch_bytes < need))
+    return fail(I8M_E_WORKSPACE, "layer_norm_backward: scratch %zu < %zu bytes", scratch ? scratch_bytes : 0, need);
+  const int groups = eight_groups(width);
+  const LnShape shape = ln_shape(width, LN_BACKWARD_OCTETS);
+  const int bands = ln_bands(rows, width);
+  float* partials = static_cast<float*>(scratch);
+  const uint8_t *c = static_cast<const uint8_t*>(codes), *e = static_cast<const uint8_t*>(exponents);
+  if (shape.octets) {
+    const bool vectors = ln_vectors(width, {dy, format < 0 ? x : codes, weight}) && on_octets(dx, dtype_size(dtype));
+    int rc = 0;
+    DISPATCH_IN(dtype, E, with_ln_shape<LN_BACKWARD_OCTETS>(shape, [&](auto family) {
+      using Family = decltype(family);
+      constexpr int V = Family::OCTETS;
+      constexpr bool WARP = Family::WARP;
+      const LnKept<E> kept{static_cast<const E*>(x), mean, c, e, groups};
+      const E *d = static_cast<const E*>(dy), *wt = static_cast<const E*>(weight);
+      float* sums_to = sums ? partials : nullptr;
+      if (!vectors) {
+        launch(ln_backward_any_kernel<E, WARP, V>, unsigned(bands), shape.block(), 0, S(stream), d, kept, rstd, wt, static_cast<E*>(dx),
+               sums_to, format, rows, width);
+        return;
+      }
+      constexpr size_t THREAD = size_t(LN_STAGES<E, WARP, V, 2>) * 2 * V * 8 * sizeof(E);
+      DISPATCH_FORMAT(format, F, {
+        auto kernel = ln_backward_kernel<E, WARP, V, F>;
+        static SmemAllowed allowed;
+        rc = allow_smem(allowed, kernel, THREAD * (WARP ? 32 * LN_WARP_ROWS : LN_BLOCK));
+        if (rc) return;
+        launch(kernel, unsigned(bands), shape.block(), THREAD * shape.block(), S(stream), d, kept, rstd, wt, static_cast<E*>(dx), sums_to,
+               rows, width);
+      });
+    }));
+    if (rc) return rc;
+    LAUNCH_CHECK("layer_norm_backward");
+  } else {
+    const long long band = (rows + bands - 1) / bands;
+    DISPATCH_IN(dtype, E, DISPATCH_FORMAT(format, F, {
+      const LnKept<E> kept{static_cast<const E*>(x), mean, c, e, groups};
+      const E* d = static_cast<const E*>(dy);
+      if (dx) {
+        launch(ln_dx_loop_kernel<E, F>, unsigned(std::min<long long>(rows, 148LL * 8)), LN_THREADS, 0, S(stream), d, kept, rstd,
+               static_cast<const E*>(weight), static_cast<E*>(dx), rows, width);
+        LAUNCH_CHECK("layer_norm_dx");
+      }
+      if (sums) {
+        launch(ln_columns_kernel<E, F>, dim3(cdiv(width, 32), bands), 32 * COLUMN_LANES, 0, S(stream), d, kept, rstd, partials,
+               rows, width, band);
+        LAUNCH_CHECK("layer_norm_columns");
+      }
+    }));
+  }
+  if (sums) {
+    DISPATCH_IN(dtype, E, (launch(column_fold_kernel<E>, dim3(cdiv(width, 32), 2), 32 * FOLD_LANES, 0, S(stream), partials,
+                                  static_cast<E*>(dweight), static_cast<E*>(dbias), width, bands)));
+    LAUNCH_CHECK("column_fold");
+  }
+  return 0;
+}

@@ -31,6 +31,12 @@ __device__ __forceinline__ uint32_t eight_exponent(uint32_t top) {
   const int e = FORMAT == EIGHT_INT8 ? int((top + 0x1ffffu) >> 23) - 6 : int((top + 0x1fffffu) >> 23) - 8;
   return uint32_t(e > 0 ? e : 0);
 }
+// max(top, |a|, |b|) in one instruction; a NaN anywhere stays one.  Its bits are what eight_exponent takes.
+__device__ __forceinline__ float top_of(float top, float a, float b) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(top), "f"(a), "f"(b));
+  return r;
+}
 // 2^-e (a normal number: bytes of finite groups end at 249; zero for the others) and 2^e.
 __device__ __forceinline__ float eight_inverse(uint32_t byte) { return __uint_as_float((254u - min(byte, 254u)) << 23); }
 __device__ __forceinline__ float eight_step(uint32_t byte) {

@@ -26,6 +26,7 @@
 //   * four TMEM buffers (all 512 columns) decouple the two sides.
 #pragma once
 #include "epi_float.cuh"
+#include "vectors.cuh"
 
 namespace i8m {
 
@@ -68,26 +69,6 @@ __device__ __forceinline__ uint8_t bq_quant(float v, float multiplier) {
     return uint8_t(((zb & 0xffu) ^ sm) - sm);                               // two's complement of the sign
   }
 }
-
-// packed two-lane FP32 arithmetic (sm_100): one issue slot for two IEEE operations
-__device__ __forceinline__ unsigned long long pack2(uint32_t lo, uint32_t hi) {
-  unsigned long long r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b,
-                                                   unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ float lane0(unsigned long long v) { return __uint_as_float(uint32_t(v)); }
-__device__ __forceinline__ float lane1(unsigned long long v) { return __uint_as_float(uint32_t(v >> 32)); }
 
 constexpr uint32_t I8_MAGIC_BITS = 0x4B400000u;  // 1.5 * 2^23 = 12582912.0f
 constexpr float I8_MAGIC = 12582912.0f;

@@ -40,10 +40,10 @@ __device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&p)[16]
 // Eight bits of one group held by one thread, stored as two 16-byte vectors and a byte.
 template <int FORMAT>
 __device__ __forceinline__ void store_group(const float (&z)[32], uint8_t* codes, uint8_t* exponent) {
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(z[j]) & 0x7fffffffu);
-  const uint32_t byte = eight_exponent<FORMAT>(top);
+  for (int j = 0; j < 32; j += 2) top = top_of(top, z[j], z[j + 1]);
+  const uint32_t byte = eight_exponent<FORMAT>(__float_as_uint(top));
   const float inverse = eight_inverse(byte);
   uint32_t c[8];
 #pragma unroll

@@ -1,7 +1,9 @@
-// Memory-bound passes of the layers around the stepped matrices: activations to and from eight bits, layer norm.
+// Memory-bound passes of the layers around the stepped matrices: activations to and from eight bits, the
+// gradient of a linear layer's pre-activation, sums over rows.
 #pragma once
 #include "activations.cuh"
 #include "eight_bit.cuh"
+#include "vectors.cuh"
 
 namespace i8m {
 
@@ -10,134 +12,146 @@ constexpr int EIGHT_THREADS = 256;
 __device__ __forceinline__ uint32_t warp_max_u(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-// One warp per group, one element per lane.  codes: (rows, 32 groups), exponents: (rows, groups).
+// Eight elements of a lane and the group that four neighbouring lanes hold: the exponent byte and the packed codes.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t quad_exponent(const float (&v)[8]) {
+  float most = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) most = top_of(most, v[j], v[j + 1]);
+  uint32_t top = __float_as_uint(most);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  return eight_exponent<FORMAT>(top);
+}
+template <int FORMAT>
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], uint32_t byte) {
+  const float inverse = eight_inverse(byte);
+  return make_uint2(eight_encode4<FORMAT>(v[0], v[1], v[2], v[3], inverse), eight_encode4<FORMAT>(v[4], v[5], v[6], v[7], inverse));
+}
+template <int FORMAT>
+__device__ __forceinline__ void decode8(uint2 codes, uint32_t byte, float (&v)[8]) {
+  const float step = eight_step(byte);
+  float lo[4], hi[4];
+  eight_decode4<FORMAT>(codes.x, step, lo);
+  eight_decode4<FORMAT>(codes.y, step, hi);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
+}
+
+// Widths of whole groups: rows follow one another without gaps, and the tensor is a list of octets (eight elements).  A
+// thread takes EIGHT_UNROLL octets, all loaded before the first is used, four neighbouring lanes hold a group.
+// Bound by HBM: 2 + 1 + 1/32 bytes per 16-bit element either way.
+constexpr int EIGHT_UNROLL = 4;
 template <typename E, int FORMAT>
 __global__ void __launch_bounds__(EIGHT_THREADS)
-eight_quant_kernel(const E* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, long long rows, int width,
-                   int groups) {
+eight_quant_octets_kernel(const E* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, long long octets) {
+  pdl_wait();
+  const long long first = (long long)blockIdx.x * (EIGHT_THREADS * EIGHT_UNROLL) + threadIdx.x;
+  float v[EIGHT_UNROLL][8];
+#pragma unroll
+  for (int u = 0; u < EIGHT_UNROLL; ++u) {
+    const long long i = first + u * EIGHT_THREADS;
+    if (i < octets) load8<E>(x + 8 * i, v[u]);
+    else for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < EIGHT_UNROLL; ++u) {
+    const long long i = first + u * EIGHT_THREADS;
+    const uint32_t byte = quad_exponent<FORMAT>(v[u]);
+    if (byte >= EightTop<E, FORMAT>::BYTE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = EightTop<E, FORMAT>::clip(v[u][j]);
+    }
+    if (i < octets) {
+      *reinterpret_cast<uint2*>(codes + 8 * i) = encode8<FORMAT>(v[u], byte);
+      if ((i & 3) == 0) exponents[i >> 2] = uint8_t(byte);
+    }
+  }
+}
+template <typename E, int FORMAT>
+__global__ void __launch_bounds__(EIGHT_THREADS)
+eight_restore_octets_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, E* __restrict__ out,
+                            long long octets) {
+  pdl_wait();
+  const long long first = (long long)blockIdx.x * (EIGHT_THREADS * EIGHT_UNROLL) + threadIdx.x;
+  uint2 c[EIGHT_UNROLL];
+  uint32_t byte[EIGHT_UNROLL];
+#pragma unroll
+  for (int u = 0; u < EIGHT_UNROLL; ++u) {
+    const long long i = first + u * EIGHT_THREADS;
+    if (i < octets) { c[u] = *reinterpret_cast<const uint2*>(codes + 8 * i); byte[u] = exponents[i >> 2]; }
+  }
+#pragma unroll
+  for (int u = 0; u < EIGHT_UNROLL; ++u) {
+    const long long i = first + u * EIGHT_THREADS;
+    float v[8];
+    if (i >= octets) continue;
+    decode8<FORMAT>(c[u], byte[u], v);
+    store8<E>(out + 8 * i, v);
+  }
+}
+
+// Any width and alignment: one element per lane, a warp takes EIGHT_SEGMENT groups of a row, four of them in flight.
+// blockIdx.y: segment of the row; rows are spread over the warps of blockIdx.x.
+constexpr int EIGHT_SEGMENT = 16;
+template <typename E, int FORMAT>
+__global__ void __launch_bounds__(EIGHT_THREADS)
+eight_quant_rows_kernel(const E* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, long long rows,
+                        int width, int groups) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long total = rows * groups;
+  const int g0 = blockIdx.y * EIGHT_SEGMENT, g1 = min(groups, g0 + EIGHT_SEGMENT);
   const long long stride = (long long)gridDim.x * (EIGHT_THREADS / 32);
-  for (long long i = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); i < total; i += stride) {
-    const long long row = i / groups;
-    const int col = int(i - row * groups) * EIGHT_GROUP + lane;
-    float v = col < width ? widen<E>(x[row * width + col]) : 0.f;
-    const uint32_t byte = eight_exponent<FORMAT>(warp_max_u(magnitude_bits(v)));
-    if (byte >= EightTop<E, FORMAT>::BYTE) v = EightTop<E, FORMAT>::clip(v);
-    codes[i * EIGHT_GROUP + lane] = eight_encode1<FORMAT>(v, eight_inverse(byte));
-    if (lane == 0) exponents[i] = uint8_t(byte);
+  for (long long row = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
+    const E* src = x + row * width + lane;
+    uint8_t* dst = codes + row * groups * EIGHT_GROUP + lane;
+    for (int g = g0; g < g1; g += EIGHT_UNROLL) {
+      float v[EIGHT_UNROLL];
+#pragma unroll
+      for (int u = 0; u < EIGHT_UNROLL; ++u) {
+        const int col = (g + u) * EIGHT_GROUP;
+        v[u] = g + u < g1 && col + lane < width ? widen<E>(src[col]) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < EIGHT_UNROLL; ++u) {
+        if (g + u >= g1) break;
+        const uint32_t byte = eight_exponent<FORMAT>(warp_max_u(magnitude_bits(v[u])));
+        if (byte >= EightTop<E, FORMAT>::BYTE) v[u] = EightTop<E, FORMAT>::clip(v[u]);
+        dst[(g + u) * EIGHT_GROUP] = eight_encode1<FORMAT>(v[u], eight_inverse(byte));
+        if (lane == 0) exponents[row * groups + g + u] = uint8_t(byte);
+      }
+    }
   }
 }
 // out: (rows, pitch); elements between width and pitch are written as zero.
 template <typename E, int FORMAT>
 __global__ void __launch_bounds__(EIGHT_THREADS)
-eight_restore_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, E* __restrict__ out, long long rows,
-                     int width, int groups, int pitch) {
+eight_restore_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, E* __restrict__ out, long long rows,
+                          int width, int groups, int pitch) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long total = rows * groups;
+  const int g0 = blockIdx.y * EIGHT_SEGMENT, g1 = min(groups, g0 + EIGHT_SEGMENT);
   const long long stride = (long long)gridDim.x * (EIGHT_THREADS / 32);
-  for (long long i = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); i < total; i += stride) {
-    const long long row = i / groups;
-    const int col = int(i - row * groups) * EIGHT_GROUP + lane;
-    const float v = eight_decode1<FORMAT>(codes[i * EIGHT_GROUP + lane], eight_step(exponents[i]));
-    if (col < pitch) out[row * pitch + col] = round_to<E>(col < width ? v : 0.f);
-  }
-}
-
-// ============================================================================ layer norm
-//   u = (x - mean) rstd,  rstd = 1 / sqrt(var + eps),  y = u w + b
-//   g = dy w,  dx = rstd (g - mean(g) - u mean(g u)),  dw = sum over rows of dy u,  db = sum over rows of dy
-// Statistics, u, g and every sum are FP32; the variance is taken around the finished mean.
-constexpr int LN_THREADS = 256;
-
-// Sum over the block, the same in every thread.
-__device__ __forceinline__ float block_total(float v, float* sh) {
+  for (long long row = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
+    const uint8_t* src = codes + row * groups * EIGHT_GROUP + lane;
+    const uint8_t* bytes = exponents + row * groups;
+    E* dst = out + row * pitch + lane;
+    for (int g = g0; g < g1; g += EIGHT_UNROLL) {
+      uint8_t c[EIGHT_UNROLL], byte[EIGHT_UNROLL];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = 0.f;
-  for (int i = 0; i < int(blockDim.x >> 5); ++i) r += sh[i];
-  __syncthreads();
-  return r;
-}
-template <typename E>
-__device__ __forceinline__ float or_else(const E* p, int i, float otherwise) { return p != nullptr ? widen<E>(p[i]) : otherwise; }
-
-// One block per row, the row read once per sweep.  FORMAT -1: no codes.
-template <typename E, int FORMAT>
-__global__ void __launch_bounds__(LN_THREADS)
-ln_forward_loop_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __restrict__ b, E* __restrict__ y,
-                       float* __restrict__ mean_out, float* __restrict__ rstd_out, uint8_t* __restrict__ codes,
-                       uint8_t* __restrict__ exponents, long long rows, int width, int groups, float eps) {
-  __shared__ float sh[LN_THREADS / 32];
-  pdl_wait();
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const E* src = x + row * width;
-    float s = 0.f;
-    for (int i = threadIdx.x; i < width; i += LN_THREADS) s += widen<E>(src[i]);
-    const float mean = block_total(s, sh) / float(width);
-    s = 0.f;
-    for (int i = threadIdx.x; i < width; i += LN_THREADS) {
-      const float d = widen<E>(src[i]) - mean;
-      s = fmaf(d, d, s);
-    }
-    const float rstd = 1.f / sqrtf(block_total(s, sh) / float(width) + eps);
-    if (threadIdx.x == 0 && mean_out != nullptr) mean_out[row] = mean;
-    if (threadIdx.x == 0 && rstd_out != nullptr) rstd_out[row] = rstd;
-    const int end = FORMAT >= 0 ? groups * EIGHT_GROUP : width;    // whole groups: warps stay together
-    for (int i = threadIdx.x; i < end; i += LN_THREADS) {
-      const float u = i < width ? (widen<E>(src[i]) - mean) * rstd : 0.f;
-      if (i < width) y[row * width + i] = round_to<E>(fmaf(u, or_else(w, i, 1.f), or_else(b, i, 0.f)));
-      if constexpr (FORMAT >= 0) {
-        const uint32_t byte = eight_exponent<FORMAT>(warp_max_u(magnitude_bits(u)));
-        codes[row * groups * EIGHT_GROUP + i] = eight_encode1<FORMAT>(u, eight_inverse(byte));
-        if ((threadIdx.x & 31) == 0) exponents[row * groups + i / EIGHT_GROUP] = uint8_t(byte);
+      for (int u = 0; u < EIGHT_UNROLL; ++u)
+        if (g + u < g1) { c[u] = src[(g + u) * EIGHT_GROUP]; byte[u] = bytes[g + u]; }
+#pragma unroll
+      for (int u = 0; u < EIGHT_UNROLL; ++u) {
+        const int col = (g + u) * EIGHT_GROUP;
+        if (g + u < g1 && col + lane < pitch)
+          dst[col] = round_to<E>(col + lane < width ? eight_decode1<FORMAT>(c[u], eight_step(byte[u])) : 0.f);
       }
     }
   }
 }
 
-// What the backward pass knows of the normalised rows: x with its rows' statistics, or the codes of u.
-template <typename E>
-struct LnKept {
-  const E* x;
-  const float* mean;
-  const uint8_t* codes;
-  const uint8_t* exponents;
-  int groups;
-};
-template <typename E, int FORMAT>
-__device__ __forceinline__ float ln_unit(const LnKept<E>& k, long long row, int width, int i, float mean, float rstd) {
-  if constexpr (FORMAT >= 0)
-    return eight_decode1<FORMAT>(k.codes[row * k.groups * EIGHT_GROUP + i], eight_step(k.exponents[row * k.groups + i / EIGHT_GROUP]));
-  else return (widen<E>(k.x[row * width + i]) - mean) * rstd;
-}
-template <typename E, int FORMAT>
-__global__ void __launch_bounds__(LN_THREADS)
-ln_dx_loop_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __restrict__ rstd_in, const E* __restrict__ w,
-                  E* __restrict__ dx, long long rows, int width) {
-  __shared__ float sh[LN_THREADS / 32];
-  pdl_wait();
-  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
-    const float mean = FORMAT >= 0 ? 0.f : kept.mean[row], rstd = rstd_in[row];
-    float sg = 0.f, su = 0.f;
-    for (int i = threadIdx.x; i < width; i += LN_THREADS) {
-      const float g = widen<E>(dy[row * width + i]) * or_else(w, i, 1.f);
-      sg += g;
-      su = fmaf(g, ln_unit<E, FORMAT>(kept, row, width, i, mean, rstd), su);
-    }
-    const float mg = block_total(sg, sh) / float(width), mu = block_total(su, sh) / float(width);
-    for (int i = threadIdx.x; i < width; i += LN_THREADS) {
-      const float g = widen<E>(dy[row * width + i]) * or_else(w, i, 1.f);
-      const float u = ln_unit<E, FORMAT>(kept, row, width, i, mean, rstd);
-      dx[row * width + i] = round_to<E>((g - mg - u * mu) * rstd);
-    }
-  }
-}
-
+// ======================================================================= sums over rows
 // Sums over rows, in two steps with a fixed order: block (c, p) adds up band p of the rows for 32 columns and leaves
 // partials (bands, 2, width); column_fold_kernel adds up the bands.
 constexpr int COLUMN_LANES = 8;      // rows that a block reads at a time
@@ -154,44 +168,26 @@ __device__ __forceinline__ void store_column_sums(float a, float b, float* parti
     partials[(size_t(blockIdx.y) * 2 + l) * width + col] = s;
   }
 }
-template <typename E, int FORMAT>
-__global__ void __launch_bounds__(32 * COLUMN_LANES)
-ln_columns_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __restrict__ rstd_in, float* __restrict__ partials,
-                  long long rows, int width, long long band) {
-  pdl_wait();
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
-  const long long first = blockIdx.y * band, last = first + band < rows ? first + band : rows;
-  float dw = 0.f, db = 0.f;
-  if (col < width) {
-    for (long long row = first + (threadIdx.x >> 5); row < last; row += COLUMN_LANES) {
-      const float v = widen<E>(dy[row * width + col]);
-      const float mean = FORMAT >= 0 ? 0.f : kept.mean[row];
-      dw = fmaf(v, ln_unit<E, FORMAT>(kept, row, width, col, mean, rstd_in[row]), dw);
-      db += v;
-    }
-  }
-  store_column_sums(dw, db, partials, width);
-}
-// out0 / out1 (either may be NULL) from partials (bands, 2, width).
+// out0 / out1 (either may be NULL) from partials (bands, 2, width): 32 columns per block, the bands spread over its warps.
+constexpr int FOLD_LANES = 16;
 template <typename E>
-__global__ void __launch_bounds__(32 * COLUMN_LANES)
+__global__ void __launch_bounds__(32 * FOLD_LANES)
 column_fold_kernel(const float* __restrict__ partials, E* __restrict__ out0, E* __restrict__ out1, int width, int bands) {
-  __shared__ float sh[2][COLUMN_LANES][32];
+  __shared__ float sh[FOLD_LANES][32];
   pdl_wait();
-  const int c = threadIdx.x & 31, l = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float s = 0.f;
-    if (col < width && (k == 0 ? out0 : out1) != nullptr)
-      for (int p = l; p < bands; p += COLUMN_LANES) s += partials[(size_t(p) * 2 + k) * width + col];
-    sh[k][l][c] = s;
+  const int c = threadIdx.x & 31, l = threadIdx.x >> 5, col = blockIdx.x * 32 + c, k = blockIdx.y;
+  E* out = k == 0 ? out0 : out1;
+  if (out == nullptr) return;                 // uniform over the block
+  float s = 0.f;
+  if (col < width) {
+#pragma unroll 4
+    for (int p = l; p < bands; p += FOLD_LANES) s += partials[(size_t(p) * 2 + k) * width + col];
   }
+  sh[l][c] = s;
   __syncthreads();
-  E* out = l == 0 ? out0 : out1;
-  if (l < 2 && col < width && out != nullptr) {
-    float s = 0.f;
+  if (l == 0 && col < width) {
 #pragma unroll
-    for (int i = 0; i < COLUMN_LANES; ++i) s += sh[l][i][c];
+    for (int i = 1; i < FOLD_LANES; ++i) s += sh[i][c];
     out[col] = round_to<E>(s);
   }
 }

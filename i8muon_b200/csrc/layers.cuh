@@ -8,9 +8,42 @@ namespace i8m {
 constexpr int MAX_LAYER_WIDTH = 1 << 24;
 constexpr long long MAX_LAYER_ROWS = 0x7fffffffLL - 1024;
 
-// Bands that sums over rows are cut into: a function of the rows alone, because the order of a sum decides its bits.
+// Bands that sums over rows are cut into: a function of the extents alone, because the order of a sum decides its bits.
 constexpr int MAX_BANDS = 296;       // two blocks per SM
 inline int row_bands(long long rows) { return int(rows < MAX_BANDS ? rows : MAX_BANDS); }
+
+// How a layer norm's rows are spread: `threads` per row (32: a warp, four rows to a block; otherwise a block) with `octets` of
+// eight elements each, at most `most` (0: wider than the kernels that hold a row in registers).
+constexpr int LN_FORWARD_OCTETS = 4, LN_BACKWARD_OCTETS = 2;
+struct LnShape {
+  int threads, octets;
+  int block() const { return threads == 32 ? 128 : threads; }
+  int rows_of_block() const { return threads == 32 ? 4 : 1; }
+  // blocks that an SM holds at one time, by the threads that the registers allow and by shared memory
+  int resident(int threads_of_sm, size_t smem) const {
+    const int by_threads = threads_of_sm / block(), by_smem = int(227 * 1024 / (smem + 1024));
+    const int n = by_threads < by_smem ? by_threads : by_smem;
+    return n < 1 ? 1 : n;
+  }
+};
+inline LnShape ln_shape(int width, int most) {
+  const int octets = width / 8 + (width % 8 != 0);
+  for (int v = 1; v <= most; v *= 2)
+    if (octets <= 32 * v) return {32, v};
+  for (int v = most; v <= 4; v *= 2)
+    if (octets <= 512 * v) return {((octets + v - 1) / v + 31) / 32 * 32, v};
+  return {0, 0};
+}
+// Bands of the backward pass's sums over rows, one per block of the register kernels: 512 resident threads per SM.
+inline int ln_bands(long long rows, int width) {
+  const LnShape s = ln_shape(width, LN_BACKWARD_OCTETS);
+  if (!s.octets) return row_bands(rows);
+  const long long blocks = (rows + s.rows_of_block() - 1) / s.rows_of_block(), most = 148LL * s.resident(512, 0);
+  return int(blocks < most ? blocks : most);
+}
+
+// Whether octets of p (rows of whole octets) lie on their own size: what vectors are stored to.
+inline bool on_octets(const void* p, size_t element) { return (reinterpret_cast<unsigned long long>(p) & (8 * element - 1)) == 0; }
 
 int eight_groups(int width);
 int eight_quant(const void* x, int dtype, long long rows, int width, int format, void* codes, void* exponents, cudaStream_t stream);

@@ -9,6 +9,7 @@
 // with --fmad=false) so that the CPU restatement reproduces them bit for bit.
 #pragma once
 #include "epi_bq.cuh"
+#include "vectors.cuh"
 
 namespace i8m {
 
@@ -59,23 +60,6 @@ __device__ __forceinline__ float block_max_256(float v, float* sh) {
 // partials of the update it writes, so that the statistics pass over it disappears): thread t takes the
 // elements 8 (t + 256 i) + e of the chunk, i = 0..3 outer, e = 0..7 inner, s = fma(v, v, s) in that order,
 // then the block tree.  Same mapping => bit-identical norms whichever kernel produced the partials.
-template <typename In>
-__device__ __forceinline__ void unpack8(const uint4 raw, float (&v)[8]) {
-  const In* e = reinterpret_cast<const In*>(&raw);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = widen<In>(e[j]);
-}
-// eight consecutive input elements (16-byte aligned): one vector load for 16-bit types, two for FP32
-template <typename In>
-__device__ __forceinline__ void load8(const In* p, float (&v)[8]) {
-  if constexpr (sizeof(In) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    unpack8<In>(*reinterpret_cast<const uint4*>(p), v);
-  }
-}
-
 // This thread's 32 elements of a chunk: four groups of eight, loaded as vectors when x allows it (all four groups in
 // flight before the first is used; with single-element loads 226 MB of BF16 took 62.7 us).
 template <typename In>
