@@ -77,13 +77,22 @@ int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width,
 
 template <typename E>
 static int linear_dz_typed(const LinearDz& d, cudaStream_t stream) {
-  const int bands = row_bands(d.rows);
+  const int bands = dz_bands(d.rows, d.width);
+  const long long band = (d.rows + bands - 1) / bands;
   const PreActivation<E> kept{static_cast<const E*>(d.z), static_cast<const uint8_t*>(d.codes),
                               static_cast<const uint8_t*>(d.exponents), d.z_pitch, eight_groups(d.width)};
-  auto kernel = d.format == EIGHT_INT8 ? linear_dz_kernel<E, EIGHT_INT8>
-              : d.format == EIGHT_E4M3 ? linear_dz_kernel<E, EIGHT_E4M3> : linear_dz_kernel<E, -1>;
-  launch(kernel, dim3(cdiv(d.width, 32), bands), 32 * COLUMN_LANES, 0, stream, static_cast<const E*>(d.dy), kept,
-         static_cast<E*>(d.dz), d.db ? d.partials : nullptr, d.rows, d.width, d.dz_pitch, (d.rows + bands - 1) / bands, d.activation);
+  float* partials = d.db ? d.partials : nullptr;
+  if (d.width % 8 == 0 && on_octets(d.dy, 2) && (d.dz == nullptr || d.dz_pitch == d.width)) {
+    auto kernel = d.format == EIGHT_INT8 ? linear_dz_octets_kernel<E, EIGHT_INT8>
+                : d.format == EIGHT_E4M3 ? linear_dz_octets_kernel<E, EIGHT_E4M3> : linear_dz_octets_kernel<E, -1>;
+    launch(kernel, dim3(cdiv(d.width, 256), bands), 32 * DZ_WARPS, 0, stream, static_cast<const E*>(d.dy), kept,
+           static_cast<E*>(d.dz), partials, d.rows, d.width, band, d.activation);
+  } else {
+    auto kernel = d.format == EIGHT_INT8 ? linear_dz_kernel<E, EIGHT_INT8>
+                : d.format == EIGHT_E4M3 ? linear_dz_kernel<E, EIGHT_E4M3> : linear_dz_kernel<E, -1>;
+    launch(kernel, dim3(cdiv(d.width, 32), bands), 32 * COLUMN_LANES, 0, stream, static_cast<const E*>(d.dy), kept,
+           static_cast<E*>(d.dz), partials, d.rows, d.width, d.dz_pitch, band, d.activation);
+  }
   LAUNCH_CHECK("linear_dz");
   if (d.db) {
     launch(column_fold_kernel<E>, cdiv(d.width, 32), 32 * FOLD_LANES, 0, stream, d.partials, static_cast<E*>(d.db),

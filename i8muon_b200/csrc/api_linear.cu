@@ -94,7 +94,7 @@ struct BackwardPieces {
     if (dx && !addressable(w_in, inner)) w = c.take(rows_bytes(outer, pitch));
     if (dw && (format >= 0 || !addressable(x_in, inner))) x = c.take(rows_bytes(rows, pitch));
     if ((dx || dw) && (activation != ACT_NONE || !addressable(dy, outer))) dz = c.take(rows_bytes(rows, pad_to(outer, 8)));
-    if (db) partials = static_cast<float*>(c.take(size_t(row_bands(rows)) * 2 * outer * sizeof(float)));
+    if (db) partials = static_cast<float*>(c.take(size_t(dz_bands(rows, outer)) * 2 * outer * sizeof(float)));
     bytes = c.used;
   }
 };

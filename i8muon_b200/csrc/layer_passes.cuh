@@ -248,4 +248,71 @@ linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict_
   if (partials != nullptr) store_column_sums(sum, 0.f, partials, width);
 }
 
+
+// The same where rows of dy, z and dz consist of whole octets on 16 bytes: a lane takes eight columns, a warp 256 of a row, the
+// block's warps rows one after the other, DZ_ROWS of them on their way at a time.  Bound by HBM (6 bytes per element, 5 with
+// codes); the special functions of an activation come second.
+constexpr int DZ_WARPS = 8, DZ_ROWS = 4;
+template <typename E, int FORMAT>
+__global__ void __launch_bounds__(32 * DZ_WARPS)
+linear_dz_octets_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict__ dz, float* __restrict__ partials,
+                        long long rows, int width, long long band, int activation) {
+  __shared__ float sums[DZ_WARPS][256];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * 8;
+  const long long first = blockIdx.y * band, last = first + band < rows ? first + band : rows;
+  unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
+  if (col < width) {
+    with_activation(activation, [&](auto act) {
+      constexpr int ACT = decltype(act)::value;
+      for (long long row = first + warp; row < last; row += DZ_WARPS * DZ_ROWS) {
+        uint4 d[DZ_ROWS], z[DZ_ROWS];
+        uint32_t byte[DZ_ROWS];
+#pragma unroll
+        for (int r = 0; r < DZ_ROWS; ++r) {
+          const long long at = row + r * DZ_WARPS;
+          if (at >= last) continue;
+          d[r] = *reinterpret_cast<const uint4*>(dy + at * width + col);
+          if constexpr (ACT == ACT_NONE) continue;
+          if constexpr (FORMAT >= 0) {
+            const uint2 c = *reinterpret_cast<const uint2*>(kept.codes + at * kept.groups * EIGHT_GROUP + col);
+            z[r].x = c.x; z[r].y = c.y;
+            byte[r] = kept.exponents[at * kept.groups + col / EIGHT_GROUP];
+          } else {
+            z[r] = *reinterpret_cast<const uint4*>(kept.z + at * kept.z_pitch + col);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < DZ_ROWS; ++r) {
+          const long long at = row + r * DZ_WARPS;
+          if (at >= last) continue;
+          float v[8];
+          unpack8<E>(d[r], v);
+          if constexpr (ACT != ACT_NONE) {
+            float f[8];
+            if constexpr (FORMAT >= 0) decode8<FORMAT>(make_uint2(z[r].x, z[r].y), byte[r], f);
+            else unpack8<E>(z[r], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= derivative<ACT>(f[j]);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[k] = add2(sum[k], pair(v[2 * k], v[2 * k + 1]));
+          if (dz != nullptr) store8<E>(dz + at * width + col, v);
+        }
+      }
+    });
+  }
+  if (partials == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) { sums[warp][8 * lane + 2 * k] = lane0(sum[k]); sums[warp][8 * lane + 2 * k + 1] = lane1(sum[k]); }
+  __syncthreads();
+  const int mine = blockIdx.x * 256 + threadIdx.x;
+  if (mine < width) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < DZ_WARPS; ++w) s += sums[w][threadIdx.x];
+    partials[size_t(blockIdx.y) * 2 * width + mine] = s;
+  }
+}
+
 }  // namespace i8m

@@ -12,6 +12,13 @@ constexpr long long MAX_LAYER_ROWS = 0x7fffffffLL - 1024;
 constexpr int MAX_BANDS = 296;       // two blocks per SM
 inline int row_bands(long long rows) { return int(rows < MAX_BANDS ? rows : MAX_BANDS); }
 
+// Bands of a linear layer's bias gradient: enough blocks of 256 columns for eight per SM, 32 rows each at least.
+inline int dz_bands(long long rows, int width) {
+  const long long columns = (width + 255) / 256, wanted = (148LL * 8 + columns - 1) / columns, most = (rows + 31) / 32;
+  const long long bands = wanted < most ? wanted : most;
+  return int(bands < MAX_BANDS ? bands : MAX_BANDS);
+}
+
 // How a layer norm's rows are spread: `threads` per row (32: a warp, four rows to a block; otherwise a block) with `octets` of
 // eight elements each, at most `most` (0: wider than the kernels that hold a row in registers).
 constexpr int LN_FORWARD_OCTETS = 4, LN_BACKWARD_OCTETS = 2;
@@ -53,7 +60,7 @@ int eight_restore(const void* codes, const void* exponents, long long rows, int 
 
 // rows of `width` 16-bit elements copied to rows of `pitch`
 int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width, int pitch, cudaStream_t stream);
-// dz = dy act'(z) into rows of dz_pitch (dz may be NULL), and db (may be NULL; partials: row_bands(rows) x 2 x width floats)
+// dz = dy act'(z) into rows of dz_pitch (dz may be NULL), and db (may be NULL; partials: dz_bands x 2 x width floats)
 struct LinearDz {
   const void* dy;
   const void* z;
