@@ -1,7 +1,10 @@
 // C ABI: linear layers (product with bias, activation and residual in the epilogue) and their backward pass.
 #include "launch_gemm.cuh"
 #include "epi_linear.cuh"
+#include "gemm_linear_split.cuh"
 #include "layers.cuh"
+
+#include <cmath>
 
 using namespace i8m;
 
@@ -12,6 +15,77 @@ struct Operand {
   const void* p;
   int pitch, mn;
 };
+
+// How a product is carried out: the 128 x 256 kernel (bn 0), or the split kernel with tiles of 128 features x bn rows.
+struct Plan {
+  int bn, split;
+};
+// The least of an estimate in nanoseconds.  128 x 256 kernel: 5 us, and per K block 0.39 us for a pair of tiles or 0.33 for one.
+// Split kernel: 4.5 us and 25 ns per column of the tile for its start, sums and end, 4 us for every further wave, and per K block
+// 14 ns for each KB that the CTA takes in, at least 0.27 us, or 17 ns per KB where two CTAs share an SM.  Both: beside the
+// time that DRAM takes for the operands (as the root of the sum of squares: neither hides the other fully).
+// Measured with BF16 operands beyond L2, in us, 128 x 256 kernel / best split (bn, CTAs per tile): 1 x 4096 -> 4096 24.7 / 10.4 (16, 4);
+// 16 x 4096 -> 14336 29.2 / 23.6 (16, 2); 128 x 4096 -> 4096 25.0 / 14.2 (64, 4); 256 25.1 / 17.3 (128, 4); 512 25.9 / 23.2
+// (128, 2); 1024 30.1 / 37.7 (128, 1); 333 x 1008 -> 520 9.0 / 6.5 (64, 4); 1024 x 768 -> 768 8.1 / 9.0 (32, 1).
+Plan plan_product(int rows, int features, int k, bool rows_mn, long long tiles, long long pairs, int sms) {
+  const int num_kb = cdiv(2LL * k, 128);
+  const double dram = 2.0 * k * ((double)rows + features) / 6200.0;
+  auto beside_dram = [&](double v) { return std::sqrt(v * v + dram * dram); };
+  const long long one = (tiles + sms - 1) / sms * num_kb * 330, two = (pairs + sms - 1) / sms * num_kb * 390;
+  Plan best{0, 1};
+  double cost = 5000 + beside_dram(double(std::min(one, two)));
+  for (int bn = rows_mn ? 64 : 16; bn <= 128; bn *= 2) {
+    const long long split_tiles = (long long)cdiv(features, TILE) * cdiv(rows, bn), kilobytes = 16 + bn / 8;
+    for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
+      // CTAs resident at one time, two per SM: GPC sizes leave some SMs out of larger clusters (148, 74, 33, 15 clusters measured)
+      const int resident = sms * 2 * (split == 4 ? 132 : split == 8 ? 120 : 148) / 148;
+      const long long ctas = split_tiles * split, waves = (ctas + resident - 1) / resident;
+      if (waves > 4) break;
+      const long long block = ctas > sms ? 17 * kilobytes : std::max<long long>(270, 14 * kilobytes);
+      const double c = 4500 + 25 * bn + 4000.0 * (waves - 1) + beside_dram(double(waves * ((num_kb + split - 1) / split) * block));
+      if (c < cost) { cost = c; best = {bn, split}; }
+    }
+    if (bn >= rows) break;
+  }
+  return best;
+}
+
+template <typename E, int BN, int A_MN, int B_MN>
+int launch_split(const CUtensorMap& ma, const CUtensorMap& mb, const LinearSplitGeom& g, const LinearArgs& args, cudaStream_t stream,
+                 const char* name) {
+  auto kernel = linear_split_kernel<E, BN, A_MN, B_MN>;
+  constexpr size_t SMEM = LinearSplitShape<BN>::SMEM;
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(allowed, kernel, SMEM)) return rc;
+  const unsigned grid = unsigned(g.tiles_f * cdiv(g.columns, BN) * g.split);
+  launch_clusters(kernel, unsigned(g.split), grid, LSP_THREADS, SMEM, stream, ma, mb, g, args);
+  LAUNCH_CHECK(name);
+  return 0;
+}
+template <typename E, int BN>
+int launch_split_layout(int f_mn, int c_mn, const CUtensorMap& ma, const CUtensorMap& mb, const LinearSplitGeom& g,
+                        const LinearArgs& args, cudaStream_t stream, const char* name) {
+  if (!f_mn) return launch_split<E, BN, 0, 0>(ma, mb, g, args, stream, name);
+  if constexpr (BN >= 64) {
+    if (c_mn) return launch_split<E, BN, 1, 1>(ma, mb, g, args, stream, name);
+  }
+  return launch_split<E, BN, 1, 0>(ma, mb, g, args, stream, name);
+}
+// out (m, n) with the split kernel: n are the features, b their operand.
+template <typename E>
+int product_split(const Plan& plan, const Operand& a, const Operand& b, int m, int n, int k, const LinearArgs& args, unsigned* status,
+                  cudaStream_t stream, const char* name) {
+  LinearSplitGeom g{n, m, cdiv(2LL * k, 128), cdiv(n, TILE), plan.split, g_starve_producers, status};
+  CUtensorMap mf, mc;
+  if (int rc = make_operand_map(&mf, b.p, 2, k, n, 1, b.mn, b.pitch)) return rc;
+  if (int rc = make_operand_map(&mc, a.p, 2, k, m, 1, a.mn, a.pitch, plan.bn)) return rc;
+  switch (plan.bn) {
+    case 16: return launch_split_layout<E, 16>(b.mn, a.mn, mf, mc, g, args, stream, name);
+    case 32: return launch_split_layout<E, 32>(b.mn, a.mn, mf, mc, g, args, stream, name);
+    case 64: return launch_split_layout<E, 64>(b.mn, a.mn, mf, mc, g, args, stream, name);
+    default: return launch_split_layout<E, 128>(b.mn, a.mn, mf, mc, g, args, stream, name);
+  }
+}
 
 // out (m, n) = a b^T over k.
 template <typename E>
@@ -29,6 +103,9 @@ int product(const Operand& a, const Operand& b, int m, int n, int k, const Linea
   g.a_mn = a.mn; g.b_mn = b.mn;
   g.group = wide_group(2LL * k);
   g.a_raw = a.p; g.b_raw = b.p; g.status = status;
+  const long long pairs = wide_units_per_batch(g.tiles_m, g.tiles_n, 0);
+  const Plan plan = plan_product(m, n, k, a.mn, tiles, pairs, sm_count());
+  if (plan.bn) return product_split<E>(plan, a, b, m, n, k, args, status, stream, name);
   CUtensorMap ma, mb;
   if (int rc = make_operand_map(&ma, a.p, 2, k, m, 1, a.mn, a.pitch)) return rc;
   if (int rc = make_operand_map(&mb, b.p, 2, k, n, 1, b.mn, b.pitch)) return rc;
@@ -36,7 +113,6 @@ int product(const Operand& a, const Operand& b, int m, int n, int k, const Linea
   auto kernel = wholek_wide_kernel<Epi>;
   static SmemAllowed allowed;
   if (int rc = allow_smem(allowed, kernel, SMEM)) return rc;
-  const long long pairs = wide_units_per_batch(g.tiles_m, g.tiles_n, 0);
   g.narrow = narrow_units(tiles, pairs, g.num_kb, sm_count());
   launch(kernel, unsigned(std::min<long long>(g.narrow ? tiles : pairs, sm_count())), WKW_THREADS, SMEM, stream, ma, mb, g, args);
   LAUNCH_CHECK(name);
