@@ -85,6 +85,10 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+
+
 def _any_gradient(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -150,10 +154,10 @@ def _norm_forward(x, weight, bias, eps, fmt, keep):
         y = torch.empty_like(x)
         mean = rstd = codes = exponents = None
         if keep:
-            rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
             if fmt == native.EIGHT_NONE:
-                mean = torch.empty_like(rstd)
+                mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
             else:
+                rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
                 codes, exponents = _empty_codes((rows,), width, x.device)
         if rows:
             native.call("i8m_layer_norm", x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd), _ptr(codes),
@@ -168,28 +172,42 @@ class _LayerNorm(torch.autograd.Function):
         x = x.contiguous()
         weight = None if weight is None else weight.contiguous()
         y, mean, rstd, codes, exponents = _norm_forward(x, weight, None if bias is None else bias.contiguous(), eps, fmt, True)
-        ctx.fmt, ctx.shape, ctx.dtype = fmt, x.shape, x.dtype
-        ctx.save_for_backward(x if fmt == native.EIGHT_NONE else None, mean, rstd, codes, exponents, weight)
+        ctx.settings = fmt, x.shape, weight is not None
+        kept = (x, mean, rstd) if fmt == native.EIGHT_NONE else (codes, exponents, rstd)
+        ctx.save_for_backward(*(kept if weight is None else (*kept, weight)))
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, mean, rstd, codes, exponents, weight = ctx.saved_tensors
-        width = ctx.shape[-1]
-        rows = dy.numel() // width
-        dy = dy.contiguous()
-        with on_device(dy.device.index):
-            make = torch.zeros if rows == 0 else torch.empty
-            dx, dw, db = (make(shape, dtype=ctx.dtype, device=dy.device) if wanted else None
-                          for wanted, shape in zip(ctx.needs_input_grad, (ctx.shape, (width,), (width,))))
-            if rows and (dx is not None or dw is not None or db is not None):
-                size = native.layer_norm_scratch_bytes(rows, width) if dw is not None or db is not None else 0
-                scratch = torch.empty(size, dtype=torch.uint8, device=dy.device) if size else None
-                native.call("i8m_layer_norm_backward", dy.data_ptr(), _ptr(x), _ptr(mean), rstd.data_ptr(), _ptr(codes),
-                            _ptr(exponents), ctx.fmt, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), rows, width,
-                            native.torch_dtype_code(ctx.dtype), _ptr(scratch), size, raw_stream(dy.device.index))
-        return dx, dw, db, None, None
+        if torch.is_grad_enabled():         # a graph of the gradients is asked for: its use is refused, not their value
+            return _norm_backward_once(ctx, dy)
+        return _norm_backward(ctx, dy)
+
+
+def _norm_backward(ctx, dy):
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    fmt, shape, scaled = ctx.settings
+    first, second, rstd, *weight = ctx.saved_tensors
+    weight = weight[0] if scaled else None
+    x, mean, codes, exponents = (first, second, None, None) if fmt == native.EIGHT_NONE else (None, None, first, second)
+    width = shape[-1]
+    dy = dy.contiguous()
+    rows, device = dy.numel() // width, dy.device
+    with on_device(device.index):
+        make = dy.new_zeros if rows == 0 else dy.new_empty
+        dx = make(shape) if need_x else None
+        dw = make((width,)) if need_w else None
+        db = make((width,)) if need_b else None
+        if rows:
+            size = native.layer_norm_scratch_bytes(rows, width) if need_w or need_b else 0
+            scratch = _workspace(size, device)
+            native.call("i8m_layer_norm_backward", dy.data_ptr(), _ptr(x), _ptr(mean), rstd.data_ptr(), _ptr(codes),
+                        _ptr(exponents), fmt, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), rows, width,
+                        native.torch_dtype_code(dy.dtype), _ptr(scratch), size, raw_stream(device.index))
+    return dx, dw, db, None, None
+
+
+_norm_backward_once = once_differentiable(_norm_backward)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5, *,
@@ -215,20 +233,16 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 
 
 # ---------------------------------------------------------------------- linear
-def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
 def _linear_forward(x, weight, bias, residual, activation, fmt, keep):
     """(y, z, codes of z, their exponents) of contiguous tensors; the last three are None where nothing is kept."""
     inner, outer = x.shape[-1], weight.shape[0]
     rows, device = x.numel() // inner, x.device
     with on_device(device.index):
-        y = torch.empty((*x.shape[:-1], outer), dtype=x.dtype, device=device)
+        y = x.new_empty((*x.shape[:-1], outer))
         z = codes = exponents = None
         if keep:
             if fmt == native.EIGHT_NONE:
-                z = torch.empty((rows, -(-outer // 8) * 8), dtype=x.dtype, device=device)
+                z = x.new_empty((rows, -(-outer // 8) * 8))
             else:
                 codes, exponents = _empty_codes((rows,), outer, device)
         if rows:
@@ -242,6 +256,12 @@ def _linear_forward(x, weight, bias, residual, activation, fmt, keep):
     return y, z, codes, exponents
 
 
+@lru_cache(maxsize=4096)
+def _backward_bytes(dy, x, weight, rows, inner, outer, activation, fmt, dx, dw, db):
+    """Workspace of a backward call; dy, x and weight are addresses modulo 16."""
+    return native.linear_backward_workspace_bytes(dy, x, weight, rows, inner, outer, activation, fmt, dx, dw, db)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, fmt):
@@ -251,39 +271,65 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         keep_z = activation != 0 and (need_x or need_w or need_b)
         y, z, z_codes, z_exponents = _linear_forward(x, weight, bias, residual, activation, fmt, keep_z)
-        x_codes = x_exponents = None
-        if need_w and fmt != native.EIGHT_NONE:
-            with on_device(x.device.index):
-                x_codes, x_exponents = _quantise(x, x.numel() // x.shape[-1], x.shape[-1], fmt, (x.numel() // x.shape[-1],))
-        ctx.activation, ctx.fmt, ctx.x_shape, ctx.w_shape, ctx.dtype = activation, fmt, x.shape, weight.shape, x.dtype
-        ctx.save_for_backward(x if need_w and fmt == native.EIGHT_NONE else None, x_codes, x_exponents,
-                              weight if need_x else None, z, z_codes, z_exponents)
+        kept = [weight] if need_x else []
+        if need_w:
+            if fmt == native.EIGHT_NONE:
+                kept.append(x)
+            else:
+                rows, inner = x.numel() // x.shape[-1], x.shape[-1]
+                with on_device(x.device.index):
+                    kept += _quantise(x, rows, inner, fmt, (rows,))
+        if keep_z:
+            kept += [z] if fmt == native.EIGHT_NONE else [z_codes, z_exponents]
+        ctx.settings = activation, fmt, x.shape, weight.shape, keep_z
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, x_codes, x_exponents, weight, z, z_codes, z_exponents = ctx.saved_tensors
-        outer, inner = ctx.w_shape
-        rows, device = dy.numel() // outer, dy.device
-        dresidual = dy if ctx.needs_input_grad[3] else None
-        dx = dw = db = None
-        if any(ctx.needs_input_grad[:3]):
-            dy = dy.contiguous()
-            with on_device(device.index):
-                make = torch.zeros if rows == 0 else torch.empty
-                dx, dw, db = (make(shape, dtype=ctx.dtype, device=device) if wanted else None
-                              for wanted, shape in zip(ctx.needs_input_grad, (ctx.x_shape, ctx.w_shape, (outer,))))
-                if rows:
-                    wants = int(dx is not None), int(dw is not None), int(db is not None)
-                    size = native.linear_backward_workspace_bytes(dy.data_ptr(), _ptr(x), _ptr(weight), rows, inner, outer,
-                                                                  ctx.activation, ctx.fmt, *wants)
-                    workspace = _workspace(size, device)
-                    native.call("i8m_linear_backward", dy.data_ptr(), _ptr(x), _ptr(x_codes), _ptr(x_exponents), _ptr(weight), _ptr(z),
-                                _ptr(z_codes), _ptr(z_exponents), ctx.fmt, ctx.activation, _ptr(dx), _ptr(dw), _ptr(db), rows,
-                                inner, outer, native.torch_dtype_code(ctx.dtype), _ptr(workspace), size,
-                                status_word(device).data_ptr(), raw_stream(device.index))
-        return dx, dw, db, dresidual, None, None
+        if torch.is_grad_enabled():         # a graph of the gradients is asked for: its use is refused, not their value
+            return _linear_backward_once(ctx, dy)
+        return _linear_backward(ctx, dy)
+
+
+def _linear_backward(ctx, dy):
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    activation, fmt, x_shape, w_shape, kept_z = ctx.settings
+    kept = iter(ctx.saved_tensors)
+    dresidual = dy if need_r else None
+    if not (need_x or need_w or need_b):
+        return None, None, None, dresidual, None, None
+    outer, inner = w_shape
+    weight = next(kept) if need_x else None
+    x = x_codes = x_exponents = z = z_codes = z_exponents = None
+    if fmt == native.EIGHT_NONE:
+        x = next(kept) if need_w else None
+        z = next(kept) if kept_z else None
+    else:
+        if need_w:
+            x_codes, x_exponents = next(kept), next(kept)
+        if kept_z:
+            z_codes, z_exponents = next(kept), next(kept)
+    dy = dy.contiguous()
+    rows, device = dy.numel() // outer, dy.device
+    with on_device(device.index):
+        make = dy.new_zeros if rows == 0 else dy.new_empty
+        dx = make(x_shape) if need_x else None
+        dw = make(w_shape) if need_w else None
+        db = make((outer,)) if need_b else None
+        if rows:
+            dy_at, x_at, w_at = dy.data_ptr(), _ptr(x), _ptr(weight)
+            size = _backward_bytes(dy_at & 15, (x_at or 0) & 15, (w_at or 0) & 15, rows, inner, outer, activation, fmt, need_x, need_w,
+                                   need_b)
+            workspace = _workspace(size, device)
+            native.call("i8m_linear_backward", dy_at, x_at, _ptr(x_codes), _ptr(x_exponents), w_at, _ptr(z), _ptr(z_codes),
+                        _ptr(z_exponents), fmt, activation, _ptr(dx), _ptr(dw), _ptr(db), rows, inner, outer,
+                        native.torch_dtype_code(dy.dtype), _ptr(workspace), size, status_word(device).data_ptr(),
+                        raw_stream(device.index))
+    return dx, dw, db, dresidual, None, None
+
+
+_linear_backward_once = once_differentiable(_linear_backward)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activation: Optional[str] = None,
