@@ -1,6 +1,6 @@
-// The activation functions of a linear layer's epilogue and their derivatives, in FP32.
+// The activation functions of a linear layer's epilogue, on pairs, and their derivatives, in FP32.
 #pragma once
-#include <cuda_runtime.h>
+#include "vectors.cuh"
 #include <type_traits>
 
 namespace i8m {
@@ -20,59 +20,83 @@ __device__ __forceinline__ float reciprocal_fast(float v) {
   return r;
 }
 constexpr float LOG2_E = 1.4426950408889634f;
-__device__ __forceinline__ float logistic(float v) { return reciprocal_fast(1.f + exp2_fast(-LOG2_E * v)); }
 
-// Normal distribution function and density.  For a = |z| and t = 1 / (1 + 0.3 a), the lower tail Phi(-a) is
-// exp(-a^2 / 2) t P(t): Phi(-a) exp(a^2 / 2) falls like 1 / a, so it is t times a smooth function, here a polynomial of degree 7
-// fitted for the least relative error over 0 <= a <= 14, where the tail leaves FP32's range: 1.5e-7 in exact arithmetic, 5e-7
-// with FP32 roundings over a grid of 200 000 points.  The exponential is the density's as well.
-struct NormalAt { float cdf, pdf; };
-__device__ __forceinline__ NormalAt normal_at(float z) {
-  const float e = exp2_fast(-0.5f * LOG2_E * z * z);
-  const float t = reciprocal_fast(fmaf(0.3f, fabsf(z), 1.f));
-  float p = 0.0356747769f;
-  p = fmaf(p, t, -0.157203108f);
-  p = fmaf(p, t, 0.20635353f);
-  p = fmaf(p, t, -0.0536836721f);
-  p = fmaf(p, t, 0.128561646f);
-  p = fmaf(p, t, 0.0999134853f);
-  p = fmaf(p, t, 0.120753959f);
-  p = fmaf(p, t, 0.119629301f);
-  const float tail = e * t * p;
-  return {z < 0.f ? tail : 1.f - tail, 0.39894228040143268f * e};
+__device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays one
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
+
+// Normal distribution: the lower tail Phi(-a) and exp(-a^2 / 2) for two a = min(|z|, 30) (beyond 14 the tail is zero in FP32).
+// With t = 1 / (1 + 0.3 a), Phi(-a) is exp(-a^2 / 2) t P(t): Phi(-a) exp(a^2 / 2) falls like 1 / a, so it is t times a smooth
+// function, here a polynomial of degree 7 fitted for the least relative error over 0 <= a <= 14: 1.5e-7 in exact arithmetic,
+// 5e-7 with FP32 roundings over a grid of 200 000 points.  Ten issue slots per element with the pairs, twenty without.
+struct NormalTail { unsigned long long tail, density; };
+__device__ __forceinline__ NormalTail normal_tail(unsigned long long a) {
+  const unsigned long long s = mul2(mul2(a, both(-0.5f * LOG2_E)), a), q = fma2(both(0.3f), a, both(1.f));
+  const unsigned long long e = pair(exp2_fast(lane0(s)), exp2_fast(lane1(s)));
+  const unsigned long long t = pair(reciprocal_fast(lane0(q)), reciprocal_fast(lane1(q)));
+  unsigned long long p = both(0.0356747769f);
+  p = fma2(p, t, both(-0.157203108f));
+  p = fma2(p, t, both(0.20635353f));
+  p = fma2(p, t, both(-0.0536836721f));
+  p = fma2(p, t, both(0.128561646f));
+  p = fma2(p, t, both(0.0999134853f));
+  p = fma2(p, t, both(0.120753959f));
+  p = fma2(p, t, both(0.119629301f));
+  return {mul2(mul2(e, t), p), e};
+}
+__device__ __forceinline__ float bounded_magnitude(float z) { return fminf(fabsf(z), 30.f); }
 
 constexpr float GELU_TANH_C = 2.f * 0.79788456080286536f;     // 2 sqrt(2 / pi)
 constexpr float GELU_TANH_K = GELU_TANH_C * 0.044715f;
 
+// 1 / (1 + 2^v) of a pair: the logistic function of -v log 2
+__device__ __forceinline__ unsigned long long gate2(unsigned long long v) {
+  const unsigned long long d = add2(pair(exp2_fast(lane0(v)), exp2_fast(lane1(v))), both(1.f));
+  return pair(reciprocal_fast(lane0(d)), reciprocal_fast(lane1(d)));
+}
 template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;              // NaN stays NaN
-  if constexpr (ACT == ACT_RELU2) return z < 0.f ? 0.f : z * z;
-  if constexpr (ACT == ACT_GELU) return z * normal_at(z).cdf;
+__device__ __forceinline__ unsigned long long activate(unsigned long long z) {
+  const float z0 = lane0(z), z1 = lane1(z);
+  if constexpr (ACT == ACT_RELU) return pair(max_nan(z0, 0.f), max_nan(z1, 0.f));
+  if constexpr (ACT == ACT_RELU2) {
+    const unsigned long long p = pair(max_nan(z0, 0.f), max_nan(z1, 0.f));
+    return mul2(p, p);
+  }
+  if constexpr (ACT == ACT_GELU) {
+    // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const unsigned long long a = pair(bounded_magnitude(z0), bounded_magnitude(z1));
+    return fma2(mul2(a, both(-1.f)), normal_tail(a).tail, pair(max_nan(z0, 0.f), max_nan(z1, 0.f)));
+  }
   // 1/2 (1 + tanh u) is the logistic function of 2 u
-  if constexpr (ACT == ACT_GELU_TANH) return z * logistic(z * fmaf(GELU_TANH_K, z * z, GELU_TANH_C));
-  if constexpr (ACT == ACT_SILU) return z * logistic(z);
+  if constexpr (ACT == ACT_GELU_TANH)
+    return mul2(z, gate2(mul2(z, fma2(both(-LOG2_E * GELU_TANH_K), mul2(z, z), both(-LOG2_E * GELU_TANH_C)))));
+  if constexpr (ACT == ACT_SILU) return mul2(z, gate2(mul2(z, both(-LOG2_E))));
   return z;
 }
 template <int ACT>
-__device__ __forceinline__ float derivative(float z) {
-  if constexpr (ACT == ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-  if constexpr (ACT == ACT_RELU2) return z < 0.f ? 0.f : 2.f * z;
+__device__ __forceinline__ unsigned long long derivative(unsigned long long z) {
+  const float z0 = lane0(z), z1 = lane1(z);
+  if constexpr (ACT == ACT_RELU) return pair(z0 > 0.f ? 1.f : (z0 <= 0.f ? 0.f : z0), z1 > 0.f ? 1.f : (z1 <= 0.f ? 0.f : z1));
+  if constexpr (ACT == ACT_RELU2) return mul2(pair(max_nan(z0, 0.f), max_nan(z1, 0.f)), both(2.f));
   if constexpr (ACT == ACT_GELU) {
-    const NormalAt n = normal_at(z);
-    return fmaf(z, n.pdf, n.cdf);
+    const NormalTail n = normal_tail(pair(bounded_magnitude(z0), bounded_magnitude(z1)));
+    const float t0 = lane0(n.tail), t1 = lane1(n.tail);
+    // the bounded z: where it differs the density is zero (and a NaN stays one)
+    const unsigned long long b = pair(max_nan(-30.f, z0 > 30.f ? 30.f : z0), max_nan(-30.f, z1 > 30.f ? 30.f : z1));
+    return fma2(mul2(b, both(0.39894228040143268f)), n.density, pair(z0 < 0.f ? t0 : 1.f - t0, z1 < 0.f ? t1 : 1.f - t1));
   }
   if constexpr (ACT == ACT_GELU_TANH) {
-    const float s = logistic(z * fmaf(GELU_TANH_K, z * z, GELU_TANH_C));
-    const float slope = fmaf(3.f * GELU_TANH_K, z * z, GELU_TANH_C);
-    return fmaf(z * s * (1.f - s), slope, s);
+    const unsigned long long q = mul2(z, z), s = gate2(mul2(z, fma2(both(-LOG2_E * GELU_TANH_K), q, both(-LOG2_E * GELU_TANH_C))));
+    const unsigned long long slope = fma2(both(3.f * GELU_TANH_K), q, both(GELU_TANH_C));
+    return fma2(mul2(mul2(z, s), fma2(s, both(-1.f), both(1.f))), slope, s);
   }
   if constexpr (ACT == ACT_SILU) {
-    const float s = logistic(z);
-    return fmaf(z * s, 1.f - s, s);
+    const unsigned long long s = gate2(mul2(z, both(-LOG2_E)));
+    return fma2(mul2(z, s), fma2(s, both(-1.f), both(1.f)), s);
   }
-  return 1.f;
+  return both(1.f);
 }
 // Calls f(std::integral_constant<int, ACT>) for the run-time code `act`.
 template <class F>

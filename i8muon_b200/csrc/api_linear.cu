@@ -1,6 +1,7 @@
 // C ABI: linear layers (product with bias, activation and residual in the epilogue) and their backward pass.
 #include "launch_gemm.cuh"
 #include "epi_linear.cuh"
+#include "gemm_linear_pair.cuh"
 #include "gemm_linear_split.cuh"
 #include "layers.cuh"
 
@@ -16,24 +17,26 @@ struct Operand {
   int pitch, mn;
 };
 
-// How a product is carried out: the 128 x 256 kernel (bn 0), or the split kernel with tiles of 128 features x bn rows.
+// How a product is carried out: on pairs of SMs in units of 256 x 256 (bn 0), or by the split kernel with tiles of 128 features x
+// bn rows.
 struct Plan {
   int bn, split;
 };
-// The least of an estimate in nanoseconds.  128 x 256 kernel: 5 us, and per K block 0.39 us for a pair of tiles or 0.33 for one.
-// Split kernel: 4.5 us and 25 ns per column of the tile for its start, sums and end, 4 us for every further wave, and per K block
-// 14 ns for each KB that the CTA takes in, at least 0.27 us, or 17 ns per KB where two CTAs share an SM.  Both: beside the
-// time that DRAM takes for the operands (as the root of the sum of squares: neither hides the other fully).
-// Measured with BF16 operands beyond L2, in us, 128 x 256 kernel / best split (bn, CTAs per tile): 1 x 4096 -> 4096 24.7 / 10.4 (16, 4);
-// 16 x 4096 -> 14336 29.2 / 23.6 (16, 2); 128 x 4096 -> 4096 25.0 / 14.2 (64, 4); 256 25.1 / 17.3 (128, 4); 512 25.9 / 23.2
-// (128, 2); 1024 30.1 / 37.7 (128, 1); 333 x 1008 -> 520 9.0 / 6.5 (64, 4); 1024 x 768 -> 768 8.1 / 9.0 (32, 1).
-Plan plan_product(int rows, int features, int k, bool rows_mn, long long tiles, long long pairs, int sms) {
+// The least of an estimate in nanoseconds.  Pairs: 6 us, and 0.365 us per K block of a wave of units.  Split kernel: 4.5 us and 25 ns
+// per column of the tile for its start, sums and end, 4 us for every further wave, and per K block 14 ns for each KB that the
+// CTA takes in, at least 0.27 us, or 17 ns per KB where two CTAs share an SM.  Both: beside the time that DRAM takes for the
+// operands (as the root of the sum of squares: neither hides the other fully).
+// Measured with BF16 operands beyond L2, in us, pairs / best split (bn, CTAs per tile): 1 x 4096 -> 4096 25 / 10.4 (16, 4);
+// 16 x 4096 -> 14336 29 / 23.6 (16, 2); 256 x 4096 -> 4096 26.6 / 17.2 (128, 4); 512 27.2 / 23.1 (128, 2); 1024 28.7 / 37.6 (128, 1);
+// 333 x 1008 -> 520 11.4 / 6.5 (64, 4); 1024 x 768 -> 768 10.2 / 9.0 (32, 1); 2048 x 1024 -> 1024 12.3 / 12.9 (64, 1);
+// 300 x 8192 -> 256 44.6 / 10.8 (64, 8).
+Plan plan_product(int rows, int features, int k, bool rows_mn, int sms) {
   const int num_kb = cdiv(2LL * k, 128);
   const double dram = 2.0 * k * ((double)rows + features) / 6200.0;
   auto beside_dram = [&](double v) { return std::sqrt(v * v + dram * dram); };
-  const long long one = (tiles + sms - 1) / sms * num_kb * 330, two = (pairs + sms - 1) / sms * num_kb * 390;
+  const long long units = (long long)cdiv(rows, 2 * TILE) * cdiv(features, 2 * TILE), pairs = std::max(1, sms / 2);
   Plan best{0, 1};
-  double cost = 5000 + beside_dram(double(std::min(one, two)));
+  double cost = 6000 + beside_dram((units + pairs - 1) / pairs * num_kb * 365.0);
   for (int bn = rows_mn ? 64 : 16; bn <= 128; bn *= 2) {
     const long long split_tiles = (long long)cdiv(features, TILE) * cdiv(rows, bn), kilobytes = 16 + bn / 8;
     for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
@@ -87,11 +90,21 @@ int product_split(const Plan& plan, const Operand& a, const Operand& b, int m, i
   }
 }
 
+template <typename E, int A_MN, int B_MN>
+int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g, const LinearArgs& args, unsigned pairs,
+                cudaStream_t stream, const char* name) {
+  auto kernel = linear_pair_kernel<E, A_MN, B_MN>;
+  static SmemAllowed allowed;
+  if (int rc = allow_smem(allowed, kernel, LPR_SMEM)) return rc;
+  launch_clusters(kernel, 2, 2 * pairs, LPR_THREADS, LPR_SMEM, stream, ma, mb, g, args);
+  LAUNCH_CHECK(name);
+  return 0;
+}
+
 // out (m, n) = a b^T over k.
 template <typename E>
 int product(const Operand& a, const Operand& b, int m, int n, int k, const LinearArgs& args, unsigned* status, cudaStream_t stream,
             const char* name) {
-  using Epi = EpiLinear<E>;
   GemmGeom g{};
   g.batch = 1; g.m = g.lm = m; g.n = g.ln = n; g.k = k;
   g.tiles_m = cdiv(m, TILE); g.tiles_n = cdiv(n, TILE);
@@ -103,20 +116,16 @@ int product(const Operand& a, const Operand& b, int m, int n, int k, const Linea
   g.a_mn = a.mn; g.b_mn = b.mn;
   g.group = wide_group(2LL * k);
   g.a_raw = a.p; g.b_raw = b.p; g.status = status;
-  const long long pairs = wide_units_per_batch(g.tiles_m, g.tiles_n, 0);
-  const Plan plan = plan_product(m, n, k, a.mn, tiles, pairs, sm_count());
+  const Plan plan = plan_product(m, n, k, a.mn, sm_count());
   if (plan.bn) return product_split<E>(plan, a, b, m, n, k, args, status, stream, name);
   CUtensorMap ma, mb;
   if (int rc = make_operand_map(&ma, a.p, 2, k, m, 1, a.mn, a.pitch)) return rc;
   if (int rc = make_operand_map(&mb, b.p, 2, k, n, 1, b.mn, b.pitch)) return rc;
-  constexpr size_t SMEM = wholek_wide_smem_bytes<Epi>();
-  auto kernel = wholek_wide_kernel<Epi>;
-  static SmemAllowed allowed;
-  if (int rc = allow_smem(allowed, kernel, SMEM)) return rc;
-  g.narrow = narrow_units(tiles, pairs, g.num_kb, sm_count());
-  launch(kernel, unsigned(std::min<long long>(g.narrow ? tiles : pairs, sm_count())), WKW_THREADS, SMEM, stream, ma, mb, g, args);
-  LAUNCH_CHECK(name);
-  return 0;
+  const long long units = (long long)cdiv(g.tiles_m, 2) * cdiv(g.tiles_n, 2);
+  const unsigned pairs_of_sms = unsigned(std::min<long long>(units, std::max(1, sm_count() / 2)));
+  if (!a.mn && !b.mn) return launch_pair<E, 0, 0>(ma, mb, g, args, pairs_of_sms, stream, name);
+  if (!a.mn) return launch_pair<E, 0, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
+  return launch_pair<E, 1, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
 }
 template <typename... A>
 int product_of(int dtype, A&&... args) {

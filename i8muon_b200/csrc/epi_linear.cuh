@@ -32,22 +32,27 @@ __device__ __forceinline__ void load_block_elements16(const WarpPatch& wp, const
 }
 
 template <typename E>
-__device__ __forceinline__ void pack_row(const float (&v)[32], uint32_t (&p)[16]) {
+__device__ __forceinline__ void pack_row(const unsigned long long (&v)[16], uint32_t (&p)[16]) {
 #pragma unroll
-  for (int k = 0; k < 16; ++k) p[k] = pack2<E>(v[2 * k], v[2 * k + 1]);
+  for (int k = 0; k < 16; ++k) p[k] = pack2<E>(lane0(v[k]), lane1(v[k]));
+}
+template <typename E>
+__device__ __forceinline__ unsigned long long widen2(uint32_t v) {
+  const float2 f = unpack2<E>(v);
+  return pair(f.x, f.y);
 }
 
 // Eight bits of one group held by one thread, stored as two 16-byte vectors and a byte.
 template <int FORMAT>
-__device__ __forceinline__ void store_group(const float (&z)[32], uint8_t* codes, uint8_t* exponent) {
+__device__ __forceinline__ void store_group(const unsigned long long (&z)[16], uint8_t* codes, uint8_t* exponent) {
   float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) top = top_of(top, z[j], z[j + 1]);
+  for (int k = 0; k < 16; ++k) top = top_of(top, lane0(z[k]), lane1(z[k]));
   const uint32_t byte = eight_exponent<FORMAT>(__float_as_uint(top));
   const float inverse = eight_inverse(byte);
   uint32_t c[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) c[j] = eight_encode4<FORMAT>(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3], inverse);
+  for (int j = 0; j < 8; ++j) c[j] = eight_encode4<FORMAT>(lane0(z[2 * j]), lane1(z[2 * j]), lane0(z[2 * j + 1]), lane1(z[2 * j + 1]), inverse);
   reinterpret_cast<uint4*>(codes)[0] = make_uint4(c[0], c[1], c[2], c[3]);
   reinterpret_cast<uint4*>(codes)[1] = make_uint4(c[4], c[5], c[6], c[7]);
   *exponent = uint8_t(byte);
@@ -76,9 +81,9 @@ struct EpiLinear {
       const int colb = t.col0 + c * 32;
       if (colb >= g.ln || wrow0 >= g.lm) continue;               // uniform over the warp
       const BlockClip clip{g.lm - wrow0, g.ln - colb};
-      float z[32];
+      unsigned long long z[16];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
+      for (int k = 0; k < 16; ++k) z[k] = pack2(v[2 * k], v[2 * k + 1]);
       if (a.bias != nullptr) {
         const E* bias = static_cast<const E*>(a.bias) + colb;
         if (clip.cols >= 32 && on_16_bytes(bias)) {
@@ -87,15 +92,12 @@ struct EpiLinear {
             const uint4 w = __ldg(reinterpret_cast<const uint4*>(bias) + q);
             const uint32_t words[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = unpack2<E>(words[k]);
-              z[8 * q + 2 * k] += f.x; z[8 * q + 2 * k + 1] += f.y;
-            }
+            for (int k = 0; k < 4; ++k) z[4 * q + k] = add2(z[4 * q + k], widen2<E>(words[k]));
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < clip.cols) z[j] += widen<E>(bias[j]);
+          for (int k = 0; k < 16; ++k)
+            z[k] = add2(z[k], pair(2 * k < clip.cols ? widen<E>(bias[2 * k]) : 0.f, 2 * k + 1 < clip.cols ? widen<E>(bias[2 * k + 1]) : 0.f));
         }
       }
       uint32_t p[16];
@@ -115,7 +117,7 @@ struct EpiLinear {
       __syncwarp();
       with_activation(a.activation, [&](auto act) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) z[j] = activate<decltype(act)::value>(z[j]);
+        for (int k = 0; k < 16; ++k) z[k] = activate<decltype(act)::value>(z[k]);
       });
       const size_t first = size_t(wrow0) * g.ln + colb;
       if (a.residual != nullptr) {
@@ -126,10 +128,7 @@ struct EpiLinear {
         wp.read_own_row(p);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 f = unpack2<E>(p[k]);
-          z[2 * k] += f.x; z[2 * k + 1] += f.y;
-        }
+        for (int k = 0; k < 16; ++k) z[k] = add2(z[k], widen2<E>(p[k]));
       }
       pack_row<E>(z, p);
       wp.write_own_row(p);

@@ -10,8 +10,8 @@
 //   warp 0       TMA producer          warp 1       tcgen05.mma issuer (M = 128, N = BN, one accumulator)
 //   warps 4..7   read the accumulator and park it       all warps   sum and epilogue
 //
-// What bounds it: reading A.  One token through 4096 x 4096 BF16 weights reads 33.6 MB; the 128 x 256 kernel has 16 units for
-// that and took 24.7 us, 32 tiles x 4 CTAs here 10.4, of which 4.5 are a launch's start, barriers and end.  Two CTAs fit on an SM (about 100 KB each), so that one streams while
+// What bounds it: reading A.  One token through 4096 x 4096 BF16 weights reads 33.6 MB; units of 256 columns are 16 for
+// that and took 25 us, 32 tiles x 4 CTAs here 10.4, of which 4.5 are a launch's start, barriers and end.  Two CTAs fit on an SM (about 100 KB each), so that one streams while
 // the other starts or ends.
 #pragma once
 #include "epi_linear.cuh"
@@ -96,8 +96,8 @@ __device__ __forceinline__ void linear_column(const LinearArgs& a, const LinearS
   }
   if (!there) return;
   with_activation(a.activation, [&](auto act) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) z[j] = activate<decltype(act)::value>(z[j]);
+    const unsigned long long y0 = activate<decltype(act)::value>(pair(z[0], z[1])), y1 = activate<decltype(act)::value>(pair(z[2], z[3]));
+    z[0] = lane0(y0); z[1] = lane1(y0); z[2] = lane0(y1); z[3] = lane1(y1);
   });
   const size_t at = size_t(c) * g.features + f;
   if (a.residual != nullptr) {

@@ -238,7 +238,7 @@ linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict_
             z = eight_decode1<FORMAT>(kept.codes[row * kept.groups * EIGHT_GROUP + col],
                                       eight_step(kept.exponents[row * kept.groups + col / EIGHT_GROUP]));
           else z = widen<E>(kept.z[row * kept.z_pitch + col]);
-          v *= derivative<ACT>(z);
+          v *= lane0(derivative<ACT>(both(z)));
         }
         sum += v;
         if (dz != nullptr) dz[row * dz_pitch + col] = round_to<E>(v);
@@ -286,17 +286,19 @@ linear_dz_octets_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __re
         for (int r = 0; r < DZ_ROWS; ++r) {
           const long long at = row + r * DZ_WARPS;
           if (at >= last) continue;
-          float v[8];
+          float v[8], f[8];
           unpack8<E>(d[r], v);
           if constexpr (ACT != ACT_NONE) {
-            float f[8];
             if constexpr (FORMAT >= 0) decode8<FORMAT>(make_uint2(z[r].x, z[r].y), byte[r], f);
             else unpack8<E>(z[r], f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= derivative<ACT>(f[j]);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum[k] = add2(sum[k], pair(v[2 * k], v[2 * k + 1]));
+          for (int k = 0; k < 4; ++k) {
+            unsigned long long p = pair(v[2 * k], v[2 * k + 1]);
+            if constexpr (ACT != ACT_NONE) p = mul2(p, derivative<ACT>(pair(f[2 * k], f[2 * k + 1])));
+            sum[k] = add2(sum[k], p);
+            v[2 * k] = lane0(p); v[2 * k + 1] = lane1(p);
+          }
           if (dz != nullptr) store8<E>(dz + at * width + col, v);
         }
       }
