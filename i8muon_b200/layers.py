@@ -89,6 +89,19 @@ def _workspace(size, device):
     return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
+_STATUS_ADDRESSES: dict = {}      # device index -> address of its status word, which stays
+
+
+def _status(device) -> int:
+    address = _STATUS_ADDRESSES.get(device.index)
+    if address is None:
+        # the word's first zeros would become part of the graph, and it would hold anything until the first replay
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("linear: make one call on this device before capturing one into a graph")
+        address = _STATUS_ADDRESSES.setdefault(device.index, status_word(device).data_ptr())
+    return address
+
+
 def _any_gradient(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -252,7 +265,7 @@ def _linear_forward(x, weight, bias, residual, activation, fmt, keep):
             workspace = _workspace(size, device)
             native.call("i8m_linear", x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z),
                         _ptr(codes), _ptr(exponents), fmt, activation, rows, inner, outer, native.torch_dtype_code(x.dtype),
-                        _ptr(workspace), size, status_word(device).data_ptr(), raw_stream(device.index))
+                        _ptr(workspace), size, _status(device), raw_stream(device.index))
     return y, z, codes, exponents
 
 
@@ -324,7 +337,7 @@ def _linear_backward(ctx, dy):
             workspace = _workspace(size, device)
             native.call("i8m_linear_backward", dy_at, x_at, _ptr(x_codes), _ptr(x_exponents), w_at, _ptr(z), _ptr(z_codes),
                         _ptr(z_exponents), fmt, activation, _ptr(dx), _ptr(dw), _ptr(db), rows, inner, outer,
-                        native.torch_dtype_code(dy.dtype), _ptr(workspace), size, status_word(device).data_ptr(),
+                        native.torch_dtype_code(dy.dtype), _ptr(workspace), size, _status(device),
                         raw_stream(device.index))
     return dx, dw, db, dresidual, None, None
 
@@ -344,7 +357,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     eight bits with ``checkpoint="int8"`` or ``"fp8"``.  The gradients are those of the formula at what was kept; the
     gradient of the pre-activation is rounded to the type of ``x`` once, as the operand of the two backward products.
 
-    A device-side wait that runs out is reported through the status word that ``check_status()`` and ``Muon.step()`` read."""
+    A device-side wait that runs out is reported through the status word that ``check_status()`` and ``Muon.step()`` read; a
+    first call on a device cannot be captured into a graph."""
     fmt = _format(checkpoint, "linear")
     if activation is not None and not isinstance(activation, str) or activation not in _ACTIVATIONS:
         raise ValueError("linear: activation must be None, 'relu', 'relu2', 'gelu', 'gelu_tanh' or 'silu'")

@@ -352,3 +352,212 @@ def test_linear_edges(cuda_device):
     with pytest.raises(RuntimeError):
         g, = torch.autograd.grad(linear(x, w).float().square().sum(), x, create_graph=True)
         g.float().sum().backward()
+
+
+# ------------------------------------------------------------- together, and as programs call them
+def block(x, p, checkpoint):
+    """A pre-norm block: norm, widening product with GELU, narrowing product onto the residual stream."""
+    u = layer_norm(x, p["nw"], p["nb"], checkpoint=checkpoint)
+    h = linear(u, p["w1"], p["b1"], activation="gelu", checkpoint=checkpoint)
+    return linear(h, p["w2"], p["b2"], residual=x, checkpoint=checkpoint)
+
+
+def block_parameters(width, dtype, device):
+    p = dict(nw=normal((width,), 1, dtype, device, 0.1, 1.0), nb=normal((width,), 2, dtype, device, 0.1),
+             w1=normal((4 * width, width), 3, dtype, device, width ** -0.5), b1=normal((4 * width,), 4, dtype, device, 0.1),
+             w2=normal((width, 4 * width), 5, dtype, device, (4 * width) ** -0.5), b2=normal((width,), 6, dtype, device, 0.1))
+    return {k: torch.nn.Parameter(v) for k, v in p.items()}
+
+
+def block_in_double(x, p, dy):
+    """The same block in 64 bits through torch's own graph: (y, gradients by name)."""
+    leaves = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    xd = x.detach().double().requires_grad_()
+    u = torch.nn.functional.layer_norm(xd, (x.shape[-1],), leaves["nw"], leaves["nb"])
+    h = torch.nn.functional.gelu(u @ leaves["w1"].t() + leaves["b1"])
+    y = h @ leaves["w2"].t() + leaves["b2"] + xd
+    g = torch.autograd.grad(y, [xd, *leaves.values()], dy.double())
+    return y, dict(zip(["x", *leaves], g))
+
+
+def relative(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+@pytest.mark.parametrize("rows, width", [(1, 64), (33, 200), (700, 256)])
+@pytest.mark.parametrize("checkpoint, loss", [(None, 0.0), ("int8", 2.0 ** -7), ("fp8", 2.0 ** -4)])
+def test_a_block_and_its_optimizer_step(cuda_device, rows, width, checkpoint, loss):
+    """Roundings on the way: the two intermediate results and the gradients between the layers are rounded to BF16, half a
+    step being 2^-8 of a value, at most six times between an input and a gradient, each of which the next product passes on
+    with its own norm; what is kept in eight bits adds up to half a step of its format (2^-7 of the group's largest value for
+    INT8, 2^-4 for E4M3) in each of the three layers."""
+    from i8muon_b200 import FusedAdamW, Muon
+    p = block_parameters(width, torch.bfloat16, cuda_device)
+    x = normal((rows, width), 9, torch.bfloat16, cuda_device).requires_grad_()
+    dy = normal((rows, width), 10, torch.bfloat16, cuda_device)
+    y = block(x, p, checkpoint)
+    want, wants = block_in_double(x, p, dy)
+    assert relative(y, want) < 3 * 2.0 ** -8
+    y.backward(dy)
+    for name, g in wants.items():
+        got = x.grad if name == "x" else p[name].grad
+        assert relative(got, g) < 6 * 2.0 ** -8 + 3 * loss, name
+    before = {k: v.detach().clone() for k, v in p.items()}
+    vectors = [p[k] for k in ("nw", "nb", "b1", "b2")]
+    Muon([p["w1"], p["w2"]], lr=0.02, precision="bfloat16", scalar_optimizer=FusedAdamW(vectors, lr=1e-2)).step()
+    check_status()
+    for k, v in p.items():
+        assert torch.isfinite(v).all() and not torch.equal(v, before[k]), k
+
+
+@pytest.mark.parametrize("rows, width", [(3, 64), (300, 200), (1500, 512)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_same_bits_twice_on_another_stream_and_replayed(cuda_device, rows, width, checkpoint):
+    dtype = torch.bfloat16
+    p = block_parameters(width, dtype, cuda_device)
+    xs = [normal((rows, width), 20 + i, dtype, cuda_device) for i in range(3)]
+    dys = [normal((rows, width), 30 + i, dtype, cuda_device) for i in range(3)]
+
+    def step(x, dy):
+        leaf = x.detach().requires_grad_()
+        y = block(leaf, p, checkpoint)
+        return [y.detach(), *torch.autograd.grad(y, [leaf, *p.values()], dy)]
+    want = [step(x, dy) for x, dy in zip(xs, dys)]
+    for a, b in zip(want[0], step(xs[0], dys[0])):
+        assert torch.equal(a, b)
+    # two streams at once
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append([step(xs[i], dys[i]) for _ in range(5)])
+    for i, s in enumerate(streams):
+        torch.cuda.current_stream().wait_stream(s)
+        for result in got[i]:
+            for a, b in zip(want[i], result):
+                assert torch.equal(a, b)
+    # captured, and replayed over other inputs in the same memory, beside an eager call
+    x, dy = xs[0].clone(), dys[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, dy)
+    for i in (1, 2, 0):
+        x.copy_(xs[i])
+        dy.copy_(dys[i])
+        graph.replay()
+        eager = step(xs[(i + 1) % 3], dys[(i + 1) % 3])
+        for a, b, c, d in zip(out, want[i], eager, want[(i + 1) % 3]):
+            assert torch.equal(a, b) and torch.equal(c, d)
+    check_status()
+
+
+def test_offsets_beyond_32_bits(cuda_device):
+    """More than 2^31 elements: the last rows of a tall tensor are what the same rows give alone."""
+    rows, width = (1 << 20) + 3, 2080
+    x = torch.zeros((rows, width), dtype=torch.bfloat16, device=cuda_device)
+    tail = normal((5, width), 1, torch.bfloat16, cuda_device)
+    x[-5:] = tail
+    assert torch.equal(restore_activation(quantise_activation(x))[-5:], restore_activation(quantise_activation(tail)))
+    leaf = x.requires_grad_()
+    y = layer_norm(leaf)
+    assert torch.equal(y[-5:], layer_norm(tail))
+    dy = torch.zeros_like(y)
+    dy[-5:] = normal((5, width), 2, torch.bfloat16, cuda_device)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    small = tail.clone().requires_grad_()
+    want, = torch.autograd.grad(layer_norm(small), small, dy[-5:])
+    assert torch.equal(dx[-5:], want) and not dx[:-5].any()
+    del y, dx, leaf, x
+    # a product with so tall a result, and its gradient
+    x = torch.zeros((rows, 64), dtype=torch.bfloat16, device=cuda_device)
+    x[-5:] = tail[:, :64]
+    w = normal((width, 64), 3, torch.bfloat16, cuda_device, 0.125).requires_grad_()
+    y = linear(x, w, activation="relu", checkpoint="int8")
+    want, tol, *_ = ref.linear(tail[:, :64].double(), w.detach().double(), None, None, "relu", torch.bfloat16)
+    ref.assert_within(y[-5:].detach(), want, tol, "y")
+    assert not y[:-5].any()
+    dw, = torch.autograd.grad(y, w, dy)
+    small = linear(x[-5:], w, activation="relu", checkpoint="int8")
+    dw_small, = torch.autograd.grad(small, w, dy[-5:])
+    # zero rows add nothing; the two calls add up in another order and may cut the sum elsewhere
+    slack = 2 * (ref.product_slack(dy[-5:].double().t(), x[-5:].double().t()) + ref.half_step(dw_small.double(), torch.bfloat16))
+    ref.assert_within(dw, dw_small.double(), slack, "dw")
+
+
+def test_only_what_belongs_to_a_tensor_is_written(cuda_device):
+    """Through the C ABI into larger buffers: a pattern around every output stays."""
+    from i8muon_b200 import native
+    from i8muon_b200.engine import status_word
+    dtype = torch.bfloat16
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def guarded(count, kind):
+        flat = torch.full((count + 512,), 77, dtype=kind, device=cuda_device)
+        return flat, flat[256:256 + count]
+
+    def intact(flat, count):
+        return bool((flat[:256] == 77).all() and (flat[256 + count:] == 77).all())
+    for rows, width, outer in ((1, 33, 7), (5, 1001, 130), (130, 72, 257), (300, 264, 513)):
+        groups, zgroups, zp = -(-width // 32), -(-outer // 32), -(-outer // 8) * 8
+        x, w = normal((rows, width), 1, dtype, cuda_device), normal((outer, width), 2, dtype, cuda_device, 0.1)
+        dy, dyx = normal((rows, outer), 3, dtype, cuda_device), normal((rows, width), 4, dtype, cuda_device)
+        sizes = dict(codes=(rows * groups * 32, torch.uint8), exps=(rows * groups, torch.uint8), back=(rows * width, dtype), y=(rows * width, dtype),
+                     dx=(rows * width, dtype), nw=(width, dtype), nb=(width, dtype), rstd=(rows, torch.float32), mean=(rows, torch.float32),
+                     ly=(rows * outer, dtype), z=(rows * zp, dtype), zcodes=(rows * zgroups * 32, torch.uint8), zexps=(rows * zgroups, torch.uint8),
+                     ldx=(rows * width, dtype), ldw=(outer * width, dtype), ldb=(outer, dtype))
+        g = {k: guarded(*v) for k, v in sizes.items()}
+        at = {k: v[1].data_ptr() for k, v in g.items()}
+        status = status_word(cuda_device).data_ptr()
+        native.call("i8m_activation_quant", x.data_ptr(), native.BF16, rows, width, 0, at["codes"], at["exps"], stream)
+        native.call("i8m_activation_restore", at["codes"], at["exps"], rows, width, 0, at["back"], native.BF16, stream)
+        native.call("i8m_layer_norm", x.data_ptr(), None, None, at["y"], at["mean"], at["rstd"], None, None, -1, rows, width, native.BF16, 1e-5, stream)
+        size = native.layer_norm_scratch_bytes(rows, width)
+        scratch = guarded(size, torch.uint8)
+        native.call("i8m_layer_norm_backward", dyx.data_ptr(), x.data_ptr(), at["mean"], at["rstd"], None, None, -1, None, at["dx"], at["nw"], at["nb"],
+                    rows, width, native.BF16, scratch[1].data_ptr(), size, stream)
+        fsize = native.linear_workspace_bytes(x.data_ptr(), w.data_ptr(), rows, width, outer)
+        fwork = guarded(fsize, torch.uint8)
+        for z, zc, ze, fmt in ((at["z"], None, None, -1), (None, at["zcodes"], at["zexps"], 1)):
+            native.call("i8m_linear", x.data_ptr(), w.data_ptr(), None, None, at["ly"], z, zc, ze, fmt, 5, rows, width, outer, native.BF16,
+                        fwork[1].data_ptr(), fsize, status, stream)
+        bsize = native.linear_backward_workspace_bytes(dy.data_ptr(), x.data_ptr(), w.data_ptr(), rows, width, outer, 5, -1, 1, 1, 1)
+        bwork = guarded(bsize, torch.uint8)
+        native.call("i8m_linear_backward", dy.data_ptr(), x.data_ptr(), None, None, w.data_ptr(), at["z"], None, None, -1, 5, at["ldx"], at["ldw"],
+                    at["ldb"], rows, width, outer, native.BF16, bwork[1].data_ptr(), bsize, status, stream)
+        torch.cuda.synchronize()
+        check_status()
+        for k, (count, _) in sizes.items():
+            assert intact(g[k][0], count), (k, rows, width, outer)
+        assert intact(scratch[0], size) and intact(fwork[0], fsize) and intact(bwork[0], bsize)
+        assert torch.equal(g["y"][1].view(rows, width), layer_norm(x))
+        assert torch.equal(g["ly"][1].view(rows, outer), linear(x, w, activation="silu"))
+
+
+@pytest.mark.parametrize("rows, inner, outer", [(3, 64, 64), (3, 1024, 512), (1100, 512, 1024)])
+def test_bounded_waits_run_out_and_report(cuda_device, rows, inner, outer):
+    """The failure path of both product kernels, in the one way that leaves nothing in flight: the producers issue no copy,
+    every other role's wait runs out after about two seconds, the status word holds a timeout code, and the same call without
+    the flag is then correct."""
+    from i8muon_b200 import native
+    x, w = normal((rows, inner), 1, torch.bfloat16, cuda_device), normal((outer, inner), 2, torch.bfloat16, cuda_device, 0.1)
+    want = linear(x, w)
+    check_status()
+    try:
+        native.call("i8m_set_debug_core", 2)
+        linear(x, w)
+        with pytest.raises(native.NativeError, match="timed out"):
+            check_status()
+    finally:
+        native.call("i8m_set_debug_core", 0)
+    assert torch.equal(linear(x, w), want)
+    check_status()
+
+
+def test_a_first_call_on_a_device_is_not_captured(cuda_device, monkeypatch):
+    from i8muon_b200 import layers
+    x, w = normal((3, 64), 1, torch.bfloat16, cuda_device), normal((64, 64), 2, torch.bfloat16, cuda_device)
+    monkeypatch.setattr(layers, "_STATUS_ADDRESSES", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        linear(x, w)
