@@ -85,8 +85,8 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
+def _workspace(size, like):
+    return like.new_empty((size,), dtype=torch.uint8) if size else None
 
 
 _STATUS_ADDRESSES: dict = {}      # device index -> address of its status word, which stays
@@ -107,19 +107,16 @@ def _any_gradient(*tensors) -> bool:
 
 
 # ------------------------------------------------------- activations in eight bits
-def _empty_codes(lead, width, device):
+def _quantise(x, rows, width, fmt, codes_at, exponents_at):
+    """A contiguous ``x`` to codes and exponents at two addresses; its device must be current."""
+    native.call("i8m_activation_quant", x.data_ptr(), native.torch_dtype_code(x.dtype), rows, width, fmt, codes_at, exponents_at,
+                raw_stream(x.device.index))
+
+
+def _eight_buffer(like, rows, width):
+    """One buffer for what a layer keeps in eight bits, codes first, and the offset of the exponents."""
     groups = -(-width // GROUP)
-    codes = torch.empty((*lead, groups * GROUP), dtype=torch.uint8, device=device)
-    return codes, torch.empty((*lead, groups), dtype=torch.uint8, device=device)
-
-
-def _quantise(x, rows, width, fmt, lead):
-    """Codes and exponents of a contiguous ``x``; its device must be current."""
-    codes, exponents = _empty_codes(lead, width, x.device)
-    if rows:
-        native.call("i8m_activation_quant", x.data_ptr(), native.torch_dtype_code(x.dtype), rows, width, fmt, codes.data_ptr(),
-                    exponents.data_ptr(), raw_stream(x.device.index))
-    return codes, exponents
+    return like.new_empty((rows * groups * (GROUP + 1),), dtype=torch.uint8), rows * groups * GROUP
 
 
 def quantise_activation(x: Tensor, checkpoint: str = "int8") -> QuantisedActivation:
@@ -130,9 +127,17 @@ def quantise_activation(x: Tensor, checkpoint: str = "int8") -> QuantisedActivat
         raise ValueError("quantise_activation: checkpoint must be 'int8' or 'fp8'")
     rows, width = _check_rows("quantise_activation", x)
     _check_device("quantise_activation", x)
+    groups = -(-width // GROUP)
+    shape = x.shape
+    if x.requires_grad:
+        x = x.detach()
+    x = x.contiguous()
     with on_device(x.device.index):
-        codes, exponents = _quantise(x.detach().contiguous(), rows, width, fmt, x.shape[:-1])
-    return QuantisedActivation(codes.view(_CODE_TYPES[fmt]), exponents, x.shape, x.dtype, checkpoint)
+        codes = x.new_empty((*shape[:-1], groups * GROUP), dtype=_CODE_TYPES[fmt])
+        exponents = x.new_empty((*shape[:-1], groups), dtype=torch.uint8)
+        if rows:
+            _quantise(x, rows, width, fmt, codes.data_ptr(), exponents.data_ptr())
+    return QuantisedActivation(codes, exponents, shape, x.dtype, checkpoint)
 
 
 def restore_activation(q: QuantisedActivation) -> Tensor:
@@ -152,7 +157,7 @@ def restore_activation(q: QuantisedActivation) -> Tensor:
     device = q.codes.device
     codes, exponents = q.codes.contiguous(), q.exponents.contiguous()
     with on_device(device.index):
-        out = torch.empty(shape, dtype=q.dtype, device=device)
+        out = codes.new_empty(shape, dtype=q.dtype)
         if out.numel():
             native.call("i8m_activation_restore", codes.data_ptr(), exponents.data_ptr(), out.numel() // width, width, fmt,
                         out.data_ptr(), native.torch_dtype_code(q.dtype), raw_stream(device.index))
@@ -161,22 +166,30 @@ def restore_activation(q: QuantisedActivation) -> Tensor:
 
 # ------------------------------------------------------------------ layer norm
 def _norm_forward(x, weight, bias, eps, fmt, keep):
-    """(y, mean, rstd, codes, exponents) of a contiguous ``x``; the last four are None where nothing is kept."""
-    rows, width = x.numel() // x.shape[-1], x.shape[-1]
-    with on_device(x.device.index):
+    """(y, statistics, what is kept in eight bits and the offset of its exponents) of a contiguous ``x``.  Statistics: the
+    rows' means and reciprocal deviations, or the latter alone beside eight bits; nothing is kept unless ``keep``."""
+    width = x.shape[-1]
+    rows, index = x.numel() // width, x.device.index
+    with on_device(index):
         y = torch.empty_like(x)
-        mean = rstd = codes = exponents = None
+        stats = eight = mean_at = rstd_at = codes_at = exponents_at = None
+        offset = 0
         if keep:
             if fmt == native.EIGHT_NONE:
-                mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind()
+                stats = x.new_empty((2, rows), dtype=torch.float32)
+                mean_at = stats.data_ptr()
+                rstd_at = mean_at + 4 * rows
             else:
-                rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-                codes, exponents = _empty_codes((rows,), width, x.device)
+                stats = x.new_empty((rows,), dtype=torch.float32)
+                rstd_at = stats.data_ptr()
+                eight, offset = _eight_buffer(x, rows, width)
+                codes_at = eight.data_ptr()
+                exponents_at = codes_at + offset
         if rows:
-            native.call("i8m_layer_norm", x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(mean), _ptr(rstd), _ptr(codes),
-                        _ptr(exponents), fmt if keep else native.EIGHT_NONE, rows, width, native.torch_dtype_code(x.dtype), eps,
-                        raw_stream(x.device.index))
-    return y, mean, rstd, codes, exponents
+            native.call("i8m_layer_norm", x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean_at, rstd_at, codes_at,
+                        exponents_at, fmt if keep else native.EIGHT_NONE, rows, width, native.torch_dtype_code(x.dtype), eps,
+                        raw_stream(index))
+    return y, stats, eight, offset
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -184,10 +197,13 @@ class _LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps, fmt):
         x = x.contiguous()
         weight = None if weight is None else weight.contiguous()
-        y, mean, rstd, codes, exponents = _norm_forward(x, weight, None if bias is None else bias.contiguous(), eps, fmt, True)
-        ctx.settings = fmt, x.shape, weight is not None
-        kept = (x, mean, rstd) if fmt == native.EIGHT_NONE else (codes, exponents, rstd)
-        ctx.save_for_backward(*(kept if weight is None else (*kept, weight)))
+        y, stats, eight, offset = _norm_forward(x, weight, None if bias is None else bias.contiguous(), eps, fmt, True)
+        ctx.settings = fmt, x.shape, offset
+        kept = x if eight is None else eight
+        if weight is None:
+            ctx.save_for_backward(kept, stats)
+        else:
+            ctx.save_for_backward(kept, stats, weight)
         return y
 
     @staticmethod
@@ -199,24 +215,27 @@ class _LayerNorm(torch.autograd.Function):
 
 def _norm_backward(ctx, dy):
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    fmt, shape, scaled = ctx.settings
-    first, second, rstd, *weight = ctx.saved_tensors
-    weight = weight[0] if scaled else None
-    x, mean, codes, exponents = (first, second, None, None) if fmt == native.EIGHT_NONE else (None, None, first, second)
+    fmt, shape, offset = ctx.settings
+    kept, stats, *weight = ctx.saved_tensors
     width = shape[-1]
     dy = dy.contiguous()
-    rows, device = dy.numel() // width, dy.device
-    with on_device(device.index):
+    rows, index = dy.numel() // width, dy.device.index
+    with on_device(index):
         make = dy.new_zeros if rows == 0 else dy.new_empty
         dx = make(shape) if need_x else None
         dw = make((width,)) if need_w else None
         db = make((width,)) if need_b else None
         if rows:
+            kept_at, stats_at = kept.data_ptr(), stats.data_ptr()
+            if fmt == native.EIGHT_NONE:
+                at = kept_at, stats_at, stats_at + 4 * rows, None, None
+            else:
+                at = None, None, stats_at, kept_at, kept_at + offset
             size = native.layer_norm_scratch_bytes(rows, width) if need_w or need_b else 0
-            scratch = _workspace(size, device)
-            native.call("i8m_layer_norm_backward", dy.data_ptr(), _ptr(x), _ptr(mean), rstd.data_ptr(), _ptr(codes),
-                        _ptr(exponents), fmt, _ptr(weight), _ptr(dx), _ptr(dw), _ptr(db), rows, width,
-                        native.torch_dtype_code(dy.dtype), _ptr(scratch), size, raw_stream(device.index))
+            scratch = _workspace(size, dy)
+            native.call("i8m_layer_norm_backward", dy.data_ptr(), *at, fmt, weight[0].data_ptr() if weight else None, _ptr(dx),
+                        _ptr(dw), _ptr(db), rows, width, native.torch_dtype_code(dy.dtype), _ptr(scratch), size,
+                        raw_stream(index))
     return dx, dw, db, None, None
 
 
@@ -241,32 +260,38 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     _check_device("layer_norm", x, weight, bias)
     if _any_gradient(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, fmt)
-    return _norm_forward(x.detach().contiguous(), None if weight is None else weight.contiguous(),
+    return _norm_forward(x.contiguous(), None if weight is None else weight.contiguous(),
                          None if bias is None else bias.contiguous(), eps, native.EIGHT_NONE, False)[0]
 
 
 # ---------------------------------------------------------------------- linear
 def _linear_forward(x, weight, bias, residual, activation, fmt, keep):
-    """(y, z, codes of z, their exponents) of contiguous tensors; the last three are None where nothing is kept."""
+    """(y, the kept pre-activation and, in eight bits, the offset of its exponents) of contiguous tensors; nothing is kept unless
+    ``keep``."""
     inner, outer = x.shape[-1], weight.shape[0]
     rows, device = x.numel() // inner, x.device
     with on_device(device.index):
         y = x.new_empty((*x.shape[:-1], outer))
-        z = codes = exponents = None
+        z = z_at = codes_at = exponents_at = None
+        offset = 0
         if keep:
             if fmt == native.EIGHT_NONE:
                 z = x.new_empty((rows, -(-outer // 8) * 8))
+                z_at = z.data_ptr()
             else:
-                codes, exponents = _empty_codes((rows,), outer, device)
+                z, offset = _eight_buffer(x, rows, outer)
+                codes_at = z.data_ptr()
+                exponents_at = codes_at + offset
         if rows:
+            x_at, w_at = x.data_ptr(), weight.data_ptr()
             size = 0
-            if inner % 8 or (x.data_ptr() | weight.data_ptr()) % 16:
-                size = native.linear_workspace_bytes(x.data_ptr(), weight.data_ptr(), rows, inner, outer)
-            workspace = _workspace(size, device)
-            native.call("i8m_linear", x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z),
-                        _ptr(codes), _ptr(exponents), fmt, activation, rows, inner, outer, native.torch_dtype_code(x.dtype),
-                        _ptr(workspace), size, _status(device), raw_stream(device.index))
-    return y, z, codes, exponents
+            if inner % 8 or (x_at | w_at) % 16:
+                size = native.linear_workspace_bytes(x_at, w_at, rows, inner, outer)
+            workspace = _workspace(size, x)
+            native.call("i8m_linear", x_at, w_at, _ptr(bias), _ptr(residual), y.data_ptr(), z_at, codes_at, exponents_at, fmt,
+                        activation, rows, inner, outer, native.torch_dtype_code(x.dtype), _ptr(workspace), size, _status(device),
+                        raw_stream(device.index))
+    return y, z, offset
 
 
 @lru_cache(maxsize=4096)
@@ -283,18 +308,23 @@ class _Linear(torch.autograd.Function):
         residual = None if residual is None else residual.contiguous()
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         keep_z = activation != 0 and (need_x or need_w or need_b)
-        y, z, z_codes, z_exponents = _linear_forward(x, weight, bias, residual, activation, fmt, keep_z)
+        y, z, z_offset = _linear_forward(x, weight, bias, residual, activation, fmt, keep_z)
         kept = [weight] if need_x else []
+        x_offset = 0
         if need_w:
             if fmt == native.EIGHT_NONE:
                 kept.append(x)
             else:
-                rows, inner = x.numel() // x.shape[-1], x.shape[-1]
+                inner = x.shape[-1]
+                rows = x.numel() // inner
                 with on_device(x.device.index):
-                    kept += _quantise(x, rows, inner, fmt, (rows,))
+                    eight, x_offset = _eight_buffer(x, rows, inner)
+                    if rows:
+                        _quantise(x, rows, inner, fmt, eight.data_ptr(), eight.data_ptr() + x_offset)
+                kept.append(eight)
         if keep_z:
-            kept += [z] if fmt == native.EIGHT_NONE else [z_codes, z_exponents]
-        ctx.settings = activation, fmt, x.shape, weight.shape, keep_z
+            kept.append(z)
+        ctx.settings = activation, fmt, x.shape, weight.shape, keep_z, x_offset, z_offset
         ctx.save_for_backward(*kept)
         return y
 
@@ -307,22 +337,15 @@ class _Linear(torch.autograd.Function):
 
 def _linear_backward(ctx, dy):
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-    activation, fmt, x_shape, w_shape, kept_z = ctx.settings
-    kept = iter(ctx.saved_tensors)
+    activation, fmt, x_shape, w_shape, kept_z, x_offset, z_offset = ctx.settings
     dresidual = dy if need_r else None
     if not (need_x or need_w or need_b):
         return None, None, None, dresidual, None, None
-    outer, inner = w_shape
+    kept = iter(ctx.saved_tensors)
     weight = next(kept) if need_x else None
-    x = x_codes = x_exponents = z = z_codes = z_exponents = None
-    if fmt == native.EIGHT_NONE:
-        x = next(kept) if need_w else None
-        z = next(kept) if kept_z else None
-    else:
-        if need_w:
-            x_codes, x_exponents = next(kept), next(kept)
-        if kept_z:
-            z_codes, z_exponents = next(kept), next(kept)
+    x = next(kept) if need_w else None
+    z = next(kept) if kept_z else None
+    outer, inner = w_shape
     dy = dy.contiguous()
     rows, device = dy.numel() // outer, dy.device
     with on_device(device.index):
@@ -331,14 +354,20 @@ def _linear_backward(ctx, dy):
         dw = make(w_shape) if need_w else None
         db = make((outer,)) if need_b else None
         if rows:
-            dy_at, x_at, w_at = dy.data_ptr(), _ptr(x), _ptr(weight)
+            dy_at, x_at, w_at, z_at = dy.data_ptr(), _ptr(x), _ptr(weight), _ptr(z)
+            # x and z, or their codes and exponents
+            x_codes = x_exponents = z_codes = z_exponents = None
+            if fmt != native.EIGHT_NONE:
+                if need_w:
+                    x_at, x_codes, x_exponents = None, x_at, x_at + x_offset
+                if kept_z:
+                    z_at, z_codes, z_exponents = None, z_at, z_at + z_offset
             size = _backward_bytes(dy_at & 15, (x_at or 0) & 15, (w_at or 0) & 15, rows, inner, outer, activation, fmt, need_x, need_w,
                                    need_b)
-            workspace = _workspace(size, device)
-            native.call("i8m_linear_backward", dy_at, x_at, _ptr(x_codes), _ptr(x_exponents), w_at, _ptr(z), _ptr(z_codes),
-                        _ptr(z_exponents), fmt, activation, _ptr(dx), _ptr(dw), _ptr(db), rows, inner, outer,
-                        native.torch_dtype_code(dy.dtype), _ptr(workspace), size, _status(device),
-                        raw_stream(device.index))
+            workspace = _workspace(size, dy)
+            native.call("i8m_linear_backward", dy_at, x_at, x_codes, x_exponents, w_at, z_at, z_codes, z_exponents, fmt, activation,
+                        _ptr(dx), _ptr(dw), _ptr(db), rows, inner, outer, native.torch_dtype_code(dy.dtype), _ptr(workspace), size,
+                        _status(device), raw_stream(device.index))
     return dx, dw, db, dresidual, None, None
 
 
@@ -373,5 +402,5 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     _check_device("linear", x, weight, bias, residual)
     if _any_gradient(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, _ACTIVATIONS[activation], fmt)
-    return _linear_forward(x.detach().contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
+    return _linear_forward(x.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous(),
                            None if residual is None else residual.contiguous(), _ACTIVATIONS[activation], native.EIGHT_NONE, False)[0]
