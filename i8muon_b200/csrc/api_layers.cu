@@ -56,8 +56,13 @@ int eight_restore(const void* codes, const void* exponents, long long rows, int 
       auto kernel = format == EIGHT_INT8 ? eight_restore_octets_kernel<Out, EIGHT_INT8> : eight_restore_octets_kernel<Out, EIGHT_E4M3>;
       launch(kernel, octet_blocks(octets), EIGHT_THREADS, 0, stream, c, e, to, octets);
     } else {
-      auto kernel = format == EIGHT_INT8 ? eight_restore_rows_kernel<Out, EIGHT_INT8> : eight_restore_rows_kernel<Out, EIGHT_E4M3>;
-      launch(kernel, row_blocks(rows, groups), EIGHT_THREADS, 0, stream, c, e, to, rows, width, groups, pitch);
+      DISPATCH_FORMAT(format, F, {
+        auto kernel = eight_restore_rows_kernel<Out, F < 0 ? EIGHT_INT8 : F, false>;
+        if constexpr (sizeof(Out) == 2) {
+          if (pitch % 8 == 0 && on_octets(out, 2)) kernel = eight_restore_rows_kernel<Out, F < 0 ? EIGHT_INT8 : F, true>;
+        }
+        launch(kernel, row_blocks(rows, groups), EIGHT_THREADS, 0, stream, c, e, to, rows, width, groups, pitch);
+      });
     }
   });
   LAUNCH_CHECK("activation_restore");
@@ -82,17 +87,12 @@ static int linear_dz_typed(const LinearDz& d, cudaStream_t stream) {
   const PreActivation<E> kept{static_cast<const E*>(d.z), static_cast<const uint8_t*>(d.codes),
                               static_cast<const uint8_t*>(d.exponents), d.z_pitch, eight_groups(d.width)};
   float* partials = d.db ? d.partials : nullptr;
-  if (d.width % 8 == 0 && on_octets(d.dy, 2) && (d.dz == nullptr || d.dz_pitch == d.width)) {
-    auto kernel = d.format == EIGHT_INT8 ? linear_dz_octets_kernel<E, EIGHT_INT8>
-                : d.format == EIGHT_E4M3 ? linear_dz_octets_kernel<E, EIGHT_E4M3> : linear_dz_octets_kernel<E, -1>;
+  const bool aligned = d.width % 8 == 0 && on_octets(d.dy, 2);
+  DISPATCH_FORMAT(d.format, F, {
+    auto kernel = aligned ? linear_dz_kernel<E, F, true> : linear_dz_kernel<E, F, false>;
     launch(kernel, dim3(cdiv(d.width, 256), bands), 32 * DZ_WARPS, 0, stream, static_cast<const E*>(d.dy), kept,
-           static_cast<E*>(d.dz), partials, d.rows, d.width, band, d.activation);
-  } else {
-    auto kernel = d.format == EIGHT_INT8 ? linear_dz_kernel<E, EIGHT_INT8>
-                : d.format == EIGHT_E4M3 ? linear_dz_kernel<E, EIGHT_E4M3> : linear_dz_kernel<E, -1>;
-    launch(kernel, dim3(cdiv(d.width, 32), bands), 32 * COLUMN_LANES, 0, stream, static_cast<const E*>(d.dy), kept,
            static_cast<E*>(d.dz), partials, d.rows, d.width, d.dz_pitch, band, d.activation);
-  }
+  });
   LAUNCH_CHECK("linear_dz");
   if (d.db) {
     launch(column_fold_kernel<E>, cdiv(d.width, 32), 32 * FOLD_LANES, 0, stream, d.partials, static_cast<E*>(d.db),
@@ -114,6 +114,7 @@ static int check_eight(const char* name, const void* a, const void* codes, const
   if (rows < 1 || width < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
   if (!float_dtype_ok(dtype)) return fail(I8M_E_ARGUMENT, "%s: bad dtype %d", name, dtype);
   if (format != EIGHT_INT8 && format != EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
+  if (reinterpret_cast<uintptr_t>(codes) & 15u) return fail(I8M_E_ARGUMENT, "%s: codes are not 16-byte aligned", name);
   if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %d is above %d", name, width, MAX_LAYER_WIDTH);
   if (rows > MAX_LAYER_ROWS) return fail(I8M_E_LIMIT, "%s: %lld rows are above %lld", name, rows, MAX_LAYER_ROWS);
   return 0;

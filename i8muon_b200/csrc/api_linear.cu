@@ -231,6 +231,8 @@ extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_
   if (dx && !weight) return fail(I8M_E_ARGUMENT, "linear_backward: dx needs the weight");
   if (dweight && (format < 0 ? !x : !x_codes || !x_exponents))
     return fail(I8M_E_ARGUMENT, "linear_backward: the weight's gradient needs x or its codes");
+  if (dweight && format >= 0 && (reinterpret_cast<uintptr_t>(x_codes) & 15u))
+    return fail(I8M_E_ARGUMENT, "linear_backward: codes of x are not 16-byte aligned");
   if (activation != ACT_NONE && (format < 0 ? !z : !z_codes || !z_exponents))
     return fail(I8M_E_ARGUMENT, "linear_backward: an activation needs z or its codes");
   if ((reinterpret_cast<uintptr_t>(z) | (format >= 0 ? reinterpret_cast<uintptr_t>(z_codes) : 0)) & 15u)

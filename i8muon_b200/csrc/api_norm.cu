@@ -17,16 +17,11 @@ int check_norm(const char* name, const void* a, const void* b, long long rows, i
   if (!float_dtype_ok(dtype)) return fail(I8M_E_ARGUMENT, "%s: bad dtype %d", name, dtype);
   if (format < -1 || format > EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
   if (format >= 0 && (!codes || !exponents)) return fail(I8M_E_ARGUMENT, "%s: null codes or exponents", name);
+  if (format >= 0 && (reinterpret_cast<uintptr_t>(codes) & 15u)) return fail(I8M_E_ARGUMENT, "%s: codes are not 16-byte aligned", name);
   if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %d is above %d", name, width, MAX_LAYER_WIDTH);
   if (rows > MAX_LAYER_ROWS) return fail(I8M_E_LIMIT, "%s: %lld rows are above %lld", name, rows, MAX_LAYER_ROWS);
   return 0;
 }
-#define DISPATCH_FORMAT(format, F, ...)                                       \
-  do {                                                                        \
-    if ((format) == EIGHT_INT8) { constexpr int F = EIGHT_INT8; __VA_ARGS__; } \
-    else if ((format) == EIGHT_E4M3) { constexpr int F = EIGHT_E4M3; __VA_ARGS__; } \
-    else { constexpr int F = -1; __VA_ARGS__; }                               \
-  } while (0)
 // Calls f(kernel family) for the shape.
 template <bool W, int V>
 struct LnFamily {

@@ -1,6 +1,7 @@
 // Layer norm, forward and backward.
 #pragma once
 #include "layer_passes.cuh"
+#include "octets.cuh"
 
 namespace i8m {
 
@@ -59,129 +60,62 @@ ln_forward_loop_kernel(const E* __restrict__ x, const E* __restrict__ w, const E
 }
 
 // ---- rows that fit into registers
-// Eight elements of a row as they lie in memory.
-template <typename E>
-struct Octet {
-  static constexpr int WORDS = int(sizeof(E)) * 2;
-  uint32_t q[WORDS];
-  // elements 2 k and 2 k + 1
-  __device__ __forceinline__ unsigned long long get(int k) const {
-    if constexpr (WORDS == 8) {
-      return pack2(q[2 * k], q[2 * k + 1]);
-    } else {
-      const float2 f = unpack2<E>(q[k]);
-      return pair(f.x, f.y);
-    }
-  }
-  __device__ __forceinline__ void load(const E* p) {          // on 16 bytes
-#pragma unroll
-    for (int k = 0; k < WORDS / 4; ++k) {
-      const uint4 w = reinterpret_cast<const uint4*>(p)[k];
-      q[4 * k] = w.x; q[4 * k + 1] = w.y; q[4 * k + 2] = w.z; q[4 * k + 3] = w.w;
-    }
-  }
-  __device__ __forceinline__ void set(int j, E v) {           // into a cleared octet
-    if constexpr (WORDS == 8) q[j] = __float_as_uint(widen<E>(v));
-    else q[j >> 1] |= uint32_t(*reinterpret_cast<const uint16_t*>(&v)) << (16 * (j & 1));
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int k = 0; k < WORDS; ++k) q[k] = 0u;
-  }
-};
-
-// The threads of a row (a warp, or the block) hold V octets each.  VEC (rows start on 16 bytes, widths of whole octets): octet v
-// of thread t is the row's octet v T + t, and a group of 32 lies in four neighbouring lanes.  Otherwise its j-th element is the
-// row's element (8 v + j) T + t, and a group lies in a warp.
+// The threads of a row (a warp, or the block) hold V octets each: octet v of thread t is the row's octet v T + t, and a group of
+// 32 lies in four neighbouring lanes.  VEC: rows start on 16 bytes (FP32 results on 32) and consist of whole octets; otherwise
+// they start anywhere, and what lies behind the width reads as zero.
 template <typename E, bool WARP, int V, bool VEC>
 struct RowSlice {
   static __device__ __forceinline__ int threads() { return WARP ? 32 : int(blockDim.x); }
-  static __device__ __forceinline__ int index(int t, int v, int j) {
-    return VEC ? 8 * (v * threads() + t) + j : (8 * v + j) * threads() + t;
-  }
-  static __device__ __forceinline__ bool inside(int t, int v, int j, int width) { return index(t, v, VEC ? 0 : j) < width; }
+  static __device__ __forceinline__ int index(int t, int v) { return 8 * (v * threads() + t); }
+  static __device__ __forceinline__ bool inside(int t, int v, int j, int width) { return index(t, v) + (VEC ? 0 : j) < width; }
   // (value, value) for the elements 2 k and 2 k + 1, zero behind the width
   static __device__ __forceinline__ unsigned long long masked(float value, int t, int v, int k, int width) {
     return pair(inside(t, v, 2 * k, width) ? value : 0.f, inside(t, v, 2 * k + 1, width) ? value : 0.f);
   }
-  static __device__ __forceinline__ void load(const E* row, int width, int t, int v, Octet<E>& o) {
-    o.clear();
+  // row of a tensor that ends at `end` (and begins at `begin`)
+  static __device__ __forceinline__ void load(const E* row, int width, int t, int v, Octet<E>& o, const E* begin, const E* end) {
     if constexpr (VEC) {
-      if (inside(t, v, 0, width)) o.load(row + index(t, v, 0));
+      o.clear();
+      if (inside(t, v, 0, width)) o.load(row + index(t, v));
     } else {
-      // every lane loads something, so that no branch stands between the loads (the row has a first element)
-      E e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = row[inside(t, v, j, width) ? index(t, v, j) : 0];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) o.set(j, inside(t, v, j, width) ? e[j] : round_to<E>(0.f));
+      load_any<E>(o, row + index(t, v), width - index(t, v), begin, end);
     }
   }
+  static __device__ __forceinline__ void load(const E* vector, int width, int t, int v, Octet<E>& o) {
+    load(vector, width, t, v, o, vector, vector + width);
+  }
+  // all lanes of the warps that hold the row call it
   static __device__ __forceinline__ void store(E* row, int width, int t, int v, const float (&x)[8]) {
     if constexpr (VEC) {
-      if (inside(t, v, 0, width)) store8<E>(row + index(t, v, 0), x);
+      if (inside(t, v, 0, width)) store8<E>(row + index(t, v), x);
     } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (inside(t, v, j, width)) row[index(t, v, j)] = round_to<E>(x[j]);
+      Octet<E> o;
+      o.pack(x);
+      store_any<E>(row + index(t, v), min(8, max(0, width - index(t, v))), o);
     }
   }
   // Eight bits of x (zero behind the width) to a row of codes and exponents; all lanes of the warps that hold the row call it.
   template <int FORMAT>
   static __device__ __forceinline__ void store_eight(uint8_t* codes, uint8_t* exponents, int groups, int t, int v, const float (&x)[8]) {
-    if constexpr (VEC) {
-      const int at = index(t, v, 0);
-      const uint32_t byte = quad_exponent<FORMAT>(x);
-      if (at < groups * EIGHT_GROUP) {
-        *reinterpret_cast<uint2*>(codes + at) = encode8<FORMAT>(x, byte);
-        if ((t & 3) == 0) exponents[at / EIGHT_GROUP] = uint8_t(byte);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = index(t, v, j);
-        const uint32_t byte = eight_exponent<FORMAT>(warp_max_u(magnitude_bits(x[j])));
-        if (at < groups * EIGHT_GROUP) {
-          codes[at] = eight_encode1<FORMAT>(x[j], eight_inverse(byte));
-          if ((t & 31) == 0) exponents[at / EIGHT_GROUP] = uint8_t(byte);
-        }
-      }
+    const int at = index(t, v);
+    const uint32_t byte = quad_exponent<FORMAT>(x);
+    if (at < groups * EIGHT_GROUP) {
+      *reinterpret_cast<uint2*>(codes + at) = encode8<FORMAT>(x, byte);
+      if ((t & 3) == 0) exponents[at / EIGHT_GROUP] = uint8_t(byte);
     }
   }
-  // Codes and exponent bytes as they lie in memory, packed into an octet's words: codes in 0 and 1, bytes in 2 (and 3).
+  // Codes and their exponent byte as they lie in memory, in an octet's words 0, 1 and 2.
   static __device__ __forceinline__ void load_eight(const uint8_t* codes, const uint8_t* exponents, int width, int t, int v, Octet<E>& o) {
     o.clear();
-    if constexpr (VEC) {
-      const int at = index(t, v, 0);
-      if (at < width) {
-        const uint2 c = *reinterpret_cast<const uint2*>(codes + at);
-        o.q[0] = c.x; o.q[1] = c.y; o.q[2] = exponents[at / EIGHT_GROUP];
-      }
-    } else {
-      uint32_t c[8], e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = inside(t, v, j, width) ? index(t, v, j) : 0;
-        c[j] = codes[at];
-        e[j] = exponents[at / EIGHT_GROUP];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (inside(t, v, j, width)) {
-          o.q[j >> 2] |= c[j] << (8 * (j & 3));
-          o.q[2 + (j >> 2)] |= e[j] << (8 * (j & 3));
-        }
+    const int at = index(t, v);
+    if (at < width) {
+      const uint2 c = *reinterpret_cast<const uint2*>(codes + at);
+      o.q[0] = c.x; o.q[1] = c.y; o.q[2] = exponents[at / EIGHT_GROUP];
     }
   }
   template <int FORMAT>
   static __device__ __forceinline__ void get_eight(const Octet<E>& o, float (&x)[8]) {
-    if constexpr (VEC) {
-      decode8<FORMAT>(make_uint2(o.q[0], o.q[1]), o.q[2], x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        x[j] = eight_decode1<FORMAT>(uint8_t(o.q[j >> 2] >> (8 * (j & 3))), eight_step(o.q[2 + (j >> 2)] >> (8 * (j & 3)) & 0xffu));
-    }
+    decode8<FORMAT>(make_uint2(o.q[0], o.q[1]), o.q[2], x);
   }
 };
 // Sums over the threads of a row (WARP: one warp, otherwise the block), the same in each: shuffles inside a warp, the warps'
@@ -268,7 +202,7 @@ ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __r
 #pragma unroll
       for (int v = 0; v < V; ++v)
         if (Slice::inside(t, v, 0, width)) {
-          const E* src = x + row * width + Slice::index(t, v, 0);
+          const E* src = x + row * width + Slice::index(t, v);
 #pragma unroll
           for (int k = 0; k < int(sizeof(E)) / 2; ++k)
             copy_async16<E>(piece(stage, v * (int(sizeof(E)) / 2) + k), reinterpret_cast<const uint8_t*>(src) + 16 * k);
@@ -307,7 +241,7 @@ ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __r
       }
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) Slice::load(x + row * width, width, t, v, in[v]);
+      for (int v = 0; v < V; ++v) Slice::load(x + row * width, width, t, v, in[v], x, x + rows * width);
     }
     unsigned long long xs[V][4], sum = 0ull;
 #pragma unroll
@@ -411,7 +345,7 @@ __device__ __forceinline__ void store_row_sums(const unsigned long long (&dw)[V]
     for (int v = 0; v < V; ++v) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int i = Slice::index(t, v, j);
+        const int i = Slice::index(t, v) + j;
         const unsigned long long a = dw[v][j / 2], c = db[v][j / 2];
         if (i < width) { line[i] = j & 1 ? lane1(a) : lane0(a); line[width + i] = j & 1 ? lane1(c) : lane0(c); }
       }
@@ -424,7 +358,7 @@ __device__ __forceinline__ void store_row_sums(const unsigned long long (&dw)[V]
         for (int v = 0; v < V; ++v) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const int i = Slice::index(t, v, j);
+            const int i = Slice::index(t, v) + j;
             const unsigned long long a = dw[v][j / 2], c = db[v][j / 2];
             sums[0][i] = (turn ? sums[0][i] : 0.f) + (j & 1 ? lane1(a) : lane0(a));
             sums[1][i] = (turn ? sums[1][i] : 0.f) + (j & 1 ? lane1(c) : lane0(c));
@@ -463,8 +397,8 @@ ln_backward_any_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __
     const float rstd = rstd_in[row], mean = format < 0 ? kept.mean[row] : 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      Slice::load(dy + row * width, width, t, v, in[v]);
-      if (format < 0) Slice::load(kept.x + row * width, width, t, v, raw[v]);
+      Slice::load(dy + row * width, width, t, v, in[v], dy, dy + rows * width);
+      if (format < 0) Slice::load(kept.x + row * width, width, t, v, raw[v], kept.x, kept.x + rows * width);
       else Slice::load_eight(kept.codes + row * kept.groups * EIGHT_GROUP, kept.exponents + row * kept.groups, width, t, v, raw[v]);
     }
     // u = the normalised row, g = dy w of octet v; behind the width dy is zero

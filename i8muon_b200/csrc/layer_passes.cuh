@@ -3,7 +3,7 @@
 #pragma once
 #include "activations.cuh"
 #include "eight_bit.cuh"
-#include "vectors.cuh"
+#include "octets.cuh"
 
 namespace i8m {
 
@@ -91,61 +91,76 @@ eight_restore_octets_kernel(const uint8_t* __restrict__ codes, const uint8_t* __
   }
 }
 
-// Any width and alignment: one element per lane, a warp takes EIGHT_SEGMENT groups of a row, four of them in flight.
-// blockIdx.y: segment of the row; rows are spread over the warps of blockIdx.x.
-constexpr int EIGHT_SEGMENT = 16;
+// Any width and alignment: a lane takes an octet, a warp 256 elements of a row at a time.  blockIdx.y: segment of the row;
+// rows are spread over the warps of blockIdx.x.
+constexpr int EIGHT_SEGMENT = 32;      // groups: four octets per lane
 template <typename E, int FORMAT>
 __global__ void __launch_bounds__(EIGHT_THREADS)
 eight_quant_rows_kernel(const E* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponents, long long rows,
                         int width, int groups) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int g0 = blockIdx.y * EIGHT_SEGMENT, g1 = min(groups, g0 + EIGHT_SEGMENT);
+  const int end = min(groups, int(blockIdx.y + 1) * EIGHT_SEGMENT) * EIGHT_GROUP;
   const long long stride = (long long)gridDim.x * (EIGHT_THREADS / 32);
   for (long long row = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
-    const E* src = x + row * width + lane;
-    uint8_t* dst = codes + row * groups * EIGHT_GROUP + lane;
-    for (int g = g0; g < g1; g += EIGHT_UNROLL) {
-      float v[EIGHT_UNROLL];
+    Octet<E> o[EIGHT_UNROLL];
 #pragma unroll
-      for (int u = 0; u < EIGHT_UNROLL; ++u) {
-        const int col = (g + u) * EIGHT_GROUP;
-        v[u] = g + u < g1 && col + lane < width ? widen<E>(src[col]) : 0.f;
+    for (int u = 0; u < EIGHT_UNROLL; ++u) {
+      const int at = int(blockIdx.y) * EIGHT_SEGMENT * EIGHT_GROUP + (u * 32 + lane) * 8;
+      load_any<E>(o[u], x + row * width + at, width - at, x, x + rows * width);
+    }
+#pragma unroll
+    for (int u = 0; u < EIGHT_UNROLL; ++u) {
+      const int at = int(blockIdx.y) * EIGHT_SEGMENT * EIGHT_GROUP + (u * 32 + lane) * 8;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { v[2 * k] = lane0(o[u].get(k)); v[2 * k + 1] = lane1(o[u].get(k)); }
+      const uint32_t byte = quad_exponent<FORMAT>(v);
+      if (byte >= EightTop<E, FORMAT>::BYTE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = EightTop<E, FORMAT>::clip(v[j]);
       }
-#pragma unroll
-      for (int u = 0; u < EIGHT_UNROLL; ++u) {
-        if (g + u >= g1) break;
-        const uint32_t byte = eight_exponent<FORMAT>(warp_max_u(magnitude_bits(v[u])));
-        if (byte >= EightTop<E, FORMAT>::BYTE) v[u] = EightTop<E, FORMAT>::clip(v[u]);
-        dst[(g + u) * EIGHT_GROUP] = eight_encode1<FORMAT>(v[u], eight_inverse(byte));
-        if (lane == 0) exponents[row * groups + g + u] = uint8_t(byte);
+      if (at < end) {
+        *reinterpret_cast<uint2*>(codes + row * groups * EIGHT_GROUP + at) = encode8<FORMAT>(v, byte);
+        if ((lane & 3) == 0) exponents[row * groups + at / EIGHT_GROUP] = uint8_t(byte);
       }
     }
   }
 }
-// out: (rows, pitch); elements between width and pitch are written as zero.
-template <typename E, int FORMAT>
+// out: (rows, pitch); elements between width and pitch are written as zero.  PITCHED: rows of out start on 16 bytes and the
+// pitch is whole octets; otherwise the pitch is the width.
+template <typename E, int FORMAT, bool PITCHED>
 __global__ void __launch_bounds__(EIGHT_THREADS)
 eight_restore_rows_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, E* __restrict__ out, long long rows,
                           int width, int groups, int pitch) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int g0 = blockIdx.y * EIGHT_SEGMENT, g1 = min(groups, g0 + EIGHT_SEGMENT);
   const long long stride = (long long)gridDim.x * (EIGHT_THREADS / 32);
   for (long long row = (long long)blockIdx.x * (EIGHT_THREADS / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
-    const uint8_t* src = codes + row * groups * EIGHT_GROUP + lane;
-    const uint8_t* bytes = exponents + row * groups;
-    E* dst = out + row * pitch + lane;
-    for (int g = g0; g < g1; g += EIGHT_UNROLL) {
-      uint8_t c[EIGHT_UNROLL], byte[EIGHT_UNROLL];
+    uint2 c[EIGHT_UNROLL];
+    uint32_t byte[EIGHT_UNROLL];
 #pragma unroll
-      for (int u = 0; u < EIGHT_UNROLL; ++u)
-        if (g + u < g1) { c[u] = src[(g + u) * EIGHT_GROUP]; byte[u] = bytes[g + u]; }
+    for (int u = 0; u < EIGHT_UNROLL; ++u) {
+      const int at = int(blockIdx.y) * EIGHT_SEGMENT * EIGHT_GROUP + (u * 32 + lane) * 8;
+      c[u] = make_uint2(0u, 0u);
+      byte[u] = 0u;
+      if (at < width) {
+        c[u] = *reinterpret_cast<const uint2*>(codes + row * groups * EIGHT_GROUP + at);
+        byte[u] = exponents[row * groups + at / EIGHT_GROUP];
+      }
+    }
 #pragma unroll
-      for (int u = 0; u < EIGHT_UNROLL; ++u) {
-        const int col = (g + u) * EIGHT_GROUP;
-        if (g + u < g1 && col + lane < pitch)
-          dst[col] = round_to<E>(col + lane < width ? eight_decode1<FORMAT>(c[u], eight_step(byte[u])) : 0.f);
+    for (int u = 0; u < EIGHT_UNROLL; ++u) {
+      const int at = int(blockIdx.y) * EIGHT_SEGMENT * EIGHT_GROUP + (u * 32 + lane) * 8;
+      float v[8];
+      decode8<FORMAT>(c[u], byte[u], v);
+      Octet<E> o;
+      o.pack(v);
+      if constexpr (PITCHED) {
+        o.cut(width - at);           // a group that reads back as NaN ends with the width
+        if (at < pitch) *reinterpret_cast<uint4*>(out + row * pitch + at) = make_uint4(o.q[0], o.q[1], o.q[2], o.q[3]);
+      } else {
+        store_any<E>(out + row * width + at, min(8, max(0, width - at)), o);
       }
     }
   }
@@ -203,10 +218,9 @@ pitch_rows_kernel(const E* __restrict__ src, E* __restrict__ dst, long long rows
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long row = i / octets;
     const int col = int(i - row * octets) * 8;
-    alignas(16) E v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = col + j < width ? src[row * width + col + j] : round_to<E>(0.f);
-    *reinterpret_cast<uint4*>(dst + row * pitch + col) = *reinterpret_cast<const uint4*>(v);
+    Octet<E> o;
+    load_any<E>(o, src + row * width + col, width - col, src, src + rows * width);
+    *reinterpret_cast<uint4*>(dst + row * pitch + col) = make_uint4(o.q[0], o.q[1], o.q[2], o.q[3]);
   }
 }
 
@@ -218,45 +232,16 @@ struct PreActivation {
   const uint8_t* exponents;
   int z_pitch, groups;
 };
-// dz = dy act'(z) (dz may be NULL) and, where partials is not NULL, its sums over bands of rows for the bias's gradient.
-template <typename E, int FORMAT>
-__global__ void __launch_bounds__(32 * COLUMN_LANES)
+// dz = dy act'(z) (dz may be NULL) and, where partials is not NULL, its sums over bands of rows for the bias's gradient: partials
+// (bands, 2, width), of which the first line of a band is written.  A lane takes eight columns, a warp 256 of a row, the
+// block's warps rows one after the other, DZ_ROWS of them on their way at a time.  ALIGNED: rows of dy are whole octets on 16
+// bytes, as those of z and dz always are.  Bound by HBM (6 bytes per element, 5 with codes); the special functions of an
+// activation come second.
+constexpr int DZ_WARPS = 8, DZ_ROWS = 4;
+template <typename E, int FORMAT, bool ALIGNED>
+__global__ void __launch_bounds__(32 * DZ_WARPS)
 linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict__ dz, float* __restrict__ partials, long long rows,
                  int width, int dz_pitch, long long band, int activation) {
-  pdl_wait();
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31);
-  const long long first = blockIdx.y * band, last = first + band < rows ? first + band : rows;
-  float sum = 0.f;
-  if (col < width) {
-    with_activation(activation, [&](auto act) {
-      constexpr int ACT = decltype(act)::value;
-      for (long long row = first + (threadIdx.x >> 5); row < last; row += COLUMN_LANES) {
-        float v = widen<E>(dy[row * width + col]);
-        if constexpr (ACT != ACT_NONE) {
-          float z;
-          if constexpr (FORMAT >= 0)
-            z = eight_decode1<FORMAT>(kept.codes[row * kept.groups * EIGHT_GROUP + col],
-                                      eight_step(kept.exponents[row * kept.groups + col / EIGHT_GROUP]));
-          else z = widen<E>(kept.z[row * kept.z_pitch + col]);
-          v *= lane0(derivative<ACT>(both(z)));
-        }
-        sum += v;
-        if (dz != nullptr) dz[row * dz_pitch + col] = round_to<E>(v);
-      }
-    });
-  }
-  if (partials != nullptr) store_column_sums(sum, 0.f, partials, width);
-}
-
-
-// The same where rows of dy, z and dz consist of whole octets on 16 bytes: a lane takes eight columns, a warp 256 of a row, the
-// block's warps rows one after the other, DZ_ROWS of them on their way at a time.  Bound by HBM (6 bytes per element, 5 with
-// codes); the special functions of an activation come second.
-constexpr int DZ_WARPS = 8, DZ_ROWS = 4;
-template <typename E, int FORMAT>
-__global__ void __launch_bounds__(32 * DZ_WARPS)
-linear_dz_octets_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict__ dz, float* __restrict__ partials,
-                        long long rows, int width, long long band, int activation) {
   __shared__ float sums[DZ_WARPS][256];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * 8;
@@ -266,13 +251,15 @@ linear_dz_octets_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __re
     with_activation(activation, [&](auto act) {
       constexpr int ACT = decltype(act)::value;
       for (long long row = first + warp; row < last; row += DZ_WARPS * DZ_ROWS) {
-        uint4 d[DZ_ROWS], z[DZ_ROWS];
+        Octet<E> d[DZ_ROWS];
+        uint4 z[DZ_ROWS];
         uint32_t byte[DZ_ROWS];
 #pragma unroll
         for (int r = 0; r < DZ_ROWS; ++r) {
           const long long at = row + r * DZ_WARPS;
           if (at >= last) continue;
-          d[r] = *reinterpret_cast<const uint4*>(dy + at * width + col);
+          if constexpr (ALIGNED) d[r].load(dy + at * width + col);
+          else load_any<E>(d[r], dy + at * width + col, width - col, dy, dy + rows * width);
           if constexpr (ACT == ACT_NONE) continue;
           if constexpr (FORMAT >= 0) {
             const uint2 c = *reinterpret_cast<const uint2*>(kept.codes + at * kept.groups * EIGHT_GROUP + col);
@@ -287,19 +274,18 @@ linear_dz_octets_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __re
           const long long at = row + r * DZ_WARPS;
           if (at >= last) continue;
           float v[8], f[8];
-          unpack8<E>(d[r], v);
           if constexpr (ACT != ACT_NONE) {
             if constexpr (FORMAT >= 0) decode8<FORMAT>(make_uint2(z[r].x, z[r].y), byte[r], f);
             else unpack8<E>(z[r], f);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            unsigned long long p = pair(v[2 * k], v[2 * k + 1]);
+            unsigned long long p = d[r].get(k);
             if constexpr (ACT != ACT_NONE) p = mul2(p, derivative<ACT>(pair(f[2 * k], f[2 * k + 1])));
             sum[k] = add2(sum[k], p);
             v[2 * k] = lane0(p); v[2 * k + 1] = lane1(p);
           }
-          if (dz != nullptr) store8<E>(dz + at * width + col, v);
+          if (dz != nullptr) store8<E>(dz + at * dz_pitch + col, v);
         }
       }
     });

@@ -2,6 +2,14 @@
 #pragma once
 #include <cuda_runtime.h>
 
+// The format as a constant: EIGHT_INT8, EIGHT_E4M3, or -1 for none.
+#define DISPATCH_FORMAT(format, F, ...)                                       \
+  do {                                                                        \
+    if ((format) == EIGHT_INT8) { constexpr int F = EIGHT_INT8; __VA_ARGS__; } \
+    else if ((format) == EIGHT_E4M3) { constexpr int F = EIGHT_E4M3; __VA_ARGS__; } \
+    else { constexpr int F = -1; __VA_ARGS__; }                               \
+  } while (0)
+
 namespace i8m {
 
 // Tensor-map coordinates and row counts of a launch are 32-bit; widths leave room for padding to 128.

@@ -156,6 +156,8 @@ def restore_activation(q: QuantisedActivation) -> Tensor:
     _check_device("restore_activation", q.codes, q.exponents)
     device = q.codes.device
     codes, exponents = q.codes.contiguous(), q.exponents.contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
     with on_device(device.index):
         out = codes.new_empty(shape, dtype=q.dtype)
         if out.numel():

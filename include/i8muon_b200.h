@@ -277,7 +277,7 @@ int i8m_adamw(void* const* params, const void* const* grads, float* const* exp_a
  * the smallest integer >= -127 with max|x| <= M 2^e, M = 127 (INT8) or 448 (E4M3); a code is x 2^-e rounded to the
  * nearest integer / E4M3 value, ties to even, and stands for code 2^e, which every dtype of x holds exactly
  * (beside the largest number of a dtype, where rounding up would leave it, the code below is taken).
- *   codes      rows x 32 ceil(width / 32) bytes, zero behind the width
+ *   codes      rows x 32 ceil(width / 32) bytes, zero behind the width; 16-byte aligned
  *   exponents  rows x ceil(width / 32) bytes e + 127; 255 marks a group that holds an infinity or a NaN and reads back as
  *              NaN throughout
  * `format` of these functions is an i8m_eight_format; where it may be I8M_EIGHT_NONE the codes are not used. */

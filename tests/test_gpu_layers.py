@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import layer_reference as ref
-from i8muon_b200 import check_status, layer_norm, linear, quantise_activation, restore_activation
+from i8muon_b200 import QuantisedActivation, check_status, layer_norm, linear, quantise_activation, restore_activation
 
 pytestmark = pytest.mark.gpu
 TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -85,6 +85,30 @@ def test_shapes_strides_and_offsets(cuda_device):
         assert got.shape == x.shape and torch.equal(got.cpu().double(), want)
     x = base.clone().requires_grad_()
     assert not quantise_activation(x, "fp8").exponents.requires_grad
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_start_at_any_element(cuda_device, dtype):
+    """Every offset from a 16-byte boundary, widths around whole octets and warps: quantised, restored and normalised."""
+    flat = normal((40000,), 3, dtype, cuda_device)
+    dyflat = normal((40000,), 4, dtype, cuda_device)
+    for width in (1, 3, 7, 8, 9, 31, 33, 39, 64, 65, 255, 257, 265, 1000, 1029, 2055):
+        rows = min(9, 16000 // width)
+        for offset in (0, 1, 2, 3, 5, 7):
+            x = flat[offset:offset + rows * width].view(rows, width)
+            q = quantise_activation(x)
+            assert torch.equal(restore_activation(q).double(), ref.kept(x.double(), "int8"))
+            w, b = flat[offset + 1:offset + 1 + width], flat[100 + offset:100 + offset + width]
+            leaf = x.detach().requires_grad_()
+            y = layer_norm(leaf, w, b)
+            want, tol, u, tol_u, rstd, rel = ref.layer_norm(x.double(), w.double(), b.double(), 1e-5, dtype)
+            ref.assert_within(y, want, tol, (width, offset))
+            dy = dyflat[2 * offset:2 * offset + rows * width].view(rows, width)
+            dx, = torch.autograd.grad(y, leaf, dy)
+            ref.assert_within(dx, *ref.layer_norm_gradients(dy.double(), u, tol_u, rstd, rel, w.double(), dtype)["dx"], (width, offset))
+    moved = QuantisedActivation(torch.zeros(97, dtype=torch.int8, device=cuda_device)[1:].copy_(q.codes[0, :96]).view(1, 96),
+                                q.exponents[:1, :3].contiguous(), torch.Size((1, 96)), dtype, "int8")
+    assert torch.equal(restore_activation(moved)[0], restore_activation(q)[0, :96])
 
 
 # ------------------------------------------------------------------ layer norm

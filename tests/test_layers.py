@@ -79,6 +79,8 @@ def test_native_argument_errors_are_codes():
     assert lib.i8m_activation_quant(16, 0, 1, 1, -1, 16, 16, None) == -1
     assert lib.i8m_activation_quant(16, 0, 1, (1 << 24) + 1, 0, 16, 16, None) == -4
     assert lib.i8m_activation_restore(16, 16, 1 << 31, 8, 0, 16, 0, None) == -4
+    assert lib.i8m_activation_quant(16, 0, 1, 1, 0, 24, 16, None) == -1        # codes on 16 bytes
+    assert lib.i8m_layer_norm(16, None, None, 16, None, None, 24, 16, 0, 1, 8, 0, 1e-5, None) == -1
     assert lib.i8m_layer_norm(16, None, None, None, None, None, None, None, -1, 1, 8, 0, 1e-5, None) == -1
     assert lib.i8m_layer_norm(16, None, None, 16, None, None, None, None, 0, 1, 8, 0, 1e-5, None) == -1
     assert lib.i8m_layer_norm(16, None, None, 16, None, None, None, None, 2, 1, 8, 0, 1e-5, None) == -1
