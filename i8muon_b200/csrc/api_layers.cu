@@ -69,13 +69,18 @@ int eight_restore(const void* codes, const void* exponents, long long rows, int 
   return 0;
 }
 
-int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width, int pitch, cudaStream_t stream) {
-  const unsigned grid = unsigned(std::min<long long>((rows * (pitch / 8) + 255) / 256, 148LL * 16));
-  if (dtype == I8M_F16)
-    launch(pitch_rows_kernel<__half>, grid, 256, 0, stream, static_cast<const __half*>(src), static_cast<__half*>(dst), rows, width, pitch);
-  else
-    launch(pitch_rows_kernel<__nv_bfloat16>, grid, 256, 0, stream, static_cast<const __nv_bfloat16*>(src),
-           static_cast<__nv_bfloat16*>(dst), rows, width, pitch);
+template <typename E>
+static void launch_pitch_rows(const void* src0, void* dst0, long long rows0, const void* src1, void* dst1, long long rows1, int width,
+                              int pitch, cudaStream_t stream) {
+  const long long octets = ((dst0 ? rows0 : 0) + (dst1 ? rows1 : 0)) * (pitch / 8);
+  launch(pitch_rows_kernel<E>, unsigned(std::min<long long>((octets + 255) / 256, 148LL * 16)), 256, 0, stream,
+         static_cast<const E*>(src0), static_cast<E*>(dst0), rows0, static_cast<const E*>(src1), static_cast<E*>(dst1), rows1, width, pitch);
+}
+int pitch_rows(const void* src0, void* dst0, long long rows0, const void* src1, void* dst1, long long rows1, int dtype, int width,
+               int pitch, cudaStream_t stream) {
+  if (!dst0 && !dst1) return 0;
+  if (dtype == I8M_F16) launch_pitch_rows<__half>(src0, dst0, rows0, src1, dst1, rows1, width, pitch, stream);
+  else launch_pitch_rows<__nv_bfloat16>(src0, dst0, rows0, src1, dst1, rows1, width, pitch, stream);
   LAUNCH_CHECK("pitch_rows");
   return 0;
 }

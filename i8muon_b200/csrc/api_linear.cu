@@ -204,8 +204,7 @@ extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, c
   if (pieces.bytes && (!workspace || workspace_bytes < pieces.bytes))
     return fail(I8M_E_WORKSPACE, "linear: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, pieces.bytes);
   const int pitch = pad_to(inner, 8);
-  if (pieces.x) { if (int rc = pitch_rows(x, pieces.x, dtype, rows, inner, pitch, S(stream))) return rc; }
-  if (pieces.w) { if (int rc = pitch_rows(weight, pieces.w, dtype, outer, inner, pitch, S(stream))) return rc; }
+  if (int rc = pitch_rows(x, pieces.x, rows, weight, pieces.w, outer, dtype, inner, pitch, S(stream))) return rc;
   LinearArgs a{};
   a.y = y; a.bias = bias; a.residual = residual;
   a.z = format < 0 ? z : nullptr; a.z_pitch = pad_to(outer, 8);
@@ -249,20 +248,19 @@ extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_
     d.dz = pieces.dz; d.dz_pitch = outer_pitch; d.db = dbias; d.partials = pieces.partials;
     if (int rc = linear_dz(d, S(stream))) return rc;
   }
+  const bool restored = format >= 0 && dweight;      // x comes from its codes
+  if (int rc = pitch_rows(x, restored ? nullptr : pieces.x, rows, weight, pieces.w, outer, dtype, inner, inner_pitch, S(stream)))
+    return rc;
   const void* dz = pieces.dz ? pieces.dz : dy;
   LinearArgs a{};
   if (dx) {
-    if (pieces.w) { if (int rc = pitch_rows(weight, pieces.w, dtype, outer, inner, inner_pitch, S(stream))) return rc; }
     a.y = dx;
     if (int rc = product_of(dtype, Operand{dz, outer_pitch, 0}, Operand{pieces.w ? pieces.w : weight, inner_pitch, 1}, rows, inner,
                             outer, a, status, S(stream), "linear_dx")) return rc;
   }
   if (dweight) {
-    if (format >= 0) {
+    if (restored)
       if (int rc = eight_restore(x_codes, x_exponents, rows, inner, format, pieces.x, dtype, inner_pitch, S(stream))) return rc;
-    } else if (pieces.x) {
-      if (int rc = pitch_rows(x, pieces.x, dtype, rows, inner, inner_pitch, S(stream))) return rc;
-    }
     a.y = dweight;
     if (int rc = product_of(dtype, Operand{dz, outer_pitch, 1}, Operand{pieces.x ? pieces.x : x, inner_pitch, 1}, outer, inner, rows,
                             a, status, S(stream), "linear_dweight")) return rc;

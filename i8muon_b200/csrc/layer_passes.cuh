@@ -209,17 +209,22 @@ column_fold_kernel(const float* __restrict__ partials, E* __restrict__ out0, E* 
 
 // ====================================================================== linear layer
 // Rows copied to a pitch that tensor copies can address (a multiple of 16 bytes).
+// Up to two matrices of the same width in one launch; dst0 or dst1 may be NULL.
 template <typename E>
 __global__ void __launch_bounds__(256)
-pitch_rows_kernel(const E* __restrict__ src, E* __restrict__ dst, long long rows, int width, int pitch) {
+pitch_rows_kernel(const E* __restrict__ src0, E* __restrict__ dst0, long long rows0, const E* __restrict__ src1, E* __restrict__ dst1,
+                  long long rows1, int width, int pitch) {
   pdl_wait();
   const int octets = pitch / 8;
-  const long long total = rows * octets;
+  const long long first = dst0 != nullptr ? rows0 * octets : 0, total = first + (dst1 != nullptr ? rows1 * octets : 0);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long row = i / octets;
-    const int col = int(i - row * octets) * 8;
+    const bool second = i >= first;
+    const E* src = second ? src1 : src0;
+    E* dst = second ? dst1 : dst0;
+    const long long at = second ? i - first : i, row = at / octets;
+    const int col = int(at - row * octets) * 8;
     Octet<E> o;
-    load_any<E>(o, src + row * width + col, width - col, src, src + rows * width);
+    load_any<E>(o, src + row * width + col, width - col, src, src + (second ? rows1 : rows0) * width);
     *reinterpret_cast<uint4*>(dst + row * pitch + col) = make_uint4(o.q[0], o.q[1], o.q[2], o.q[3]);
   }
 }

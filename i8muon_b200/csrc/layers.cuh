@@ -66,8 +66,9 @@ int eight_quant(const void* x, int dtype, long long rows, int width, int format,
 int eight_restore(const void* codes, const void* exponents, long long rows, int width, int format, void* out, int dtype, int pitch,
                   cudaStream_t stream);
 
-// rows of `width` 16-bit elements copied to rows of `pitch`
-int pitch_rows(const void* src, void* dst, int dtype, long long rows, int width, int pitch, cudaStream_t stream);
+// rows of `width` 16-bit elements copied to rows of `pitch`, of one or two matrices (a dst that is NULL is left out)
+int pitch_rows(const void* src0, void* dst0, long long rows0, const void* src1, void* dst1, long long rows1, int dtype, int width,
+               int pitch, cudaStream_t stream);
 // dz = dy act'(z) into rows of dz_pitch (dz may be NULL), and db (may be NULL; partials: dz_bands x 2 x width floats)
 struct LinearDz {
   const void* dy;
