@@ -62,12 +62,12 @@ extern "C" int i8m_layer_norm(const void* x, const void* weight, const void* bia
     DISPATCH_IN(dtype, E, with_ln_shape<LN_FORWARD_OCTETS>(shape, [&](auto family) {
       using Family = decltype(family);
       constexpr int V = Family::OCTETS;
-      auto kernel = vectors ? ln_forward_kernel<E, Family::WARP, V, true> : ln_forward_kernel<E, Family::WARP, V, false>;
+      auto kernel = vectors ? ln_forward_kernel<E, Family::WARP, V, false> : ln_forward_kernel<E, Family::WARP, V, true>;
       const int block = shape.block();
       constexpr size_t STAGES = LN_STAGES<E, Family::WARP, V, 1>;
-      const size_t smem = vectors ? STAGES * block * V * 8 * sizeof(E) : 0;
-      static SmemAllowed allowed;
-      if (vectors) rc = allow_smem(allowed, kernel, STAGES * ln_stage_bytes<E, Family::WARP, V>(1));
+      const size_t smem = STAGES * (block * V * 8 * sizeof(E) + (vectors ? 0 : 16 * shape.rows_of_block()));
+      static SmemAllowed allowed[2];
+      rc = allow_smem(allowed[vectors], kernel, STAGES * (ln_stage_bytes<E, Family::WARP, V>(1) + 16 * LN_WARP_ROWS));
       if (rc) return;
       launch(kernel, unsigned(std::min<long long>(cdiv(rows, shape.rows_of_block()), 148LL * shape.resident(512, smem))), block, smem, S(stream),
              static_cast<const E*>(x), static_cast<const E*>(weight), static_cast<const E*>(bias), static_cast<E*>(y), mean, rstd,
@@ -112,19 +112,14 @@ extern "C" int i8m_layer_norm_backward(const void* dy, const void* x, const floa
       const LnKept<E> kept{static_cast<const E*>(x), mean, c, e, groups};
       const E *d = static_cast<const E*>(dy), *wt = static_cast<const E*>(weight);
       float* sums_to = sums ? partials : nullptr;
-      if (!vectors) {
-        launch(ln_backward_any_kernel<E, WARP, V>, unsigned(bands), shape.block(), 0, S(stream), d, kept, rstd, wt, static_cast<E*>(dx),
-               sums_to, format, rows, width);
-        return;
-      }
-      constexpr size_t THREAD = size_t(LN_STAGES<E, WARP, V, 2>) * 2 * V * 8 * sizeof(E);
+      constexpr size_t STAGES = LN_STAGES<E, WARP, V, 2>, THREAD = STAGES * 2 * V * 8 * sizeof(E);
+      const size_t smem = THREAD * shape.block() + (vectors ? 0 : STAGES * 2 * 16 * shape.rows_of_block());
       DISPATCH_FORMAT(format, F, {
-        auto kernel = ln_backward_kernel<E, WARP, V, F>;
-        static SmemAllowed allowed;
-        rc = allow_smem(allowed, kernel, THREAD * (WARP ? 32 * LN_WARP_ROWS : LN_BLOCK));
+        auto kernel = vectors ? ln_backward_kernel<E, WARP, V, F, false> : ln_backward_kernel<E, WARP, V, F, true>;
+        static SmemAllowed allowed[2];
+        rc = allow_smem(allowed[vectors], kernel, THREAD * (WARP ? 32 * LN_WARP_ROWS : LN_BLOCK) + STAGES * 2 * 16 * LN_WARP_ROWS);
         if (rc) return;
-        launch(kernel, unsigned(bands), shape.block(), THREAD * shape.block(), S(stream), d, kept, rstd, wt, static_cast<E*>(dx), sums_to,
-               rows, width);
+        launch(kernel, unsigned(bands), shape.block(), smem, S(stream), d, kept, rstd, wt, static_cast<E*>(dx), sums_to, rows, width);
       });
     }));
     if (rc) return rc;

@@ -104,19 +104,6 @@ struct RowSlice {
       if ((t & 3) == 0) exponents[at / EIGHT_GROUP] = uint8_t(byte);
     }
   }
-  // Codes and their exponent byte as they lie in memory, in an octet's words 0, 1 and 2.
-  static __device__ __forceinline__ void load_eight(const uint8_t* codes, const uint8_t* exponents, int width, int t, int v, Octet<E>& o) {
-    o.clear();
-    const int at = index(t, v);
-    if (at < width) {
-      const uint2 c = *reinterpret_cast<const uint2*>(codes + at);
-      o.q[0] = c.x; o.q[1] = c.y; o.q[2] = exponents[at / EIGHT_GROUP];
-    }
-  }
-  template <int FORMAT>
-  static __device__ __forceinline__ void get_eight(const Octet<E>& o, float (&x)[8]) {
-    decode8<FORMAT>(make_uint2(o.q[0], o.q[1]), o.q[2], x);
-  }
 };
 // Sums over the threads of a row (WARP: one warp, otherwise the block), the same in each: shuffles inside a warp, the warps'
 // sums through shared memory.  One barrier: the caller alternates between two buffers.
@@ -180,54 +167,120 @@ template <typename E, bool WARP, int V, int INPUTS>
 constexpr int LN_STAGES = 4 * ln_stage_bytes<E, WARP, V>(INPUTS) <= 208 * 1024 ? 4
                         : 3 * ln_stage_bytes<E, WARP, V>(INPUTS) <= 208 * 1024 ? 3 : 1;
 
+// A row that starts anywhere on its way through shared memory: the aligned 16-byte pieces that hold it, in order, copied by all
+// threads of the row and read at the row's offset.  What lies outside the tensor (a first or last piece) is left out.
+template <typename E, bool WARP, int V>
+struct ShiftedRow {
+  static constexpr int PIECES = int(sizeof(E)) / 2;
+  static __device__ __forceinline__ int threads() { return WARP ? 32 : int(blockDim.x); }
+  static __device__ __forceinline__ uint32_t bytes() { return uint32_t(threads() * V * PIECES + 1) * 16u; }
+  static __device__ __forceinline__ void piece(const E* row, int width, int c, const E* begin, const E* end, uint32_t to) {
+    const uintptr_t at = (reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15)) + 16u * uint32_t(c);
+    if (at >= reinterpret_cast<uintptr_t>(row + width)) return;
+    to += 16u * uint32_t(c);
+    if (at >= reinterpret_cast<uintptr_t>(begin) && at + 16u <= reinterpret_cast<uintptr_t>(end)) {
+      copy_async16<__half>(to, reinterpret_cast<const void*>(at));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16 / int(sizeof(E)); ++j) {
+        const E* e = reinterpret_cast<const E*>(at) + j;
+        if (e < begin || e >= end) continue;
+        if constexpr (sizeof(E) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + 4u * j), "f"(widen<E>(*e)) : "memory");
+        else asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + 2u * j), "h"(*reinterpret_cast<const uint16_t*>(e)) : "memory");
+      }
+    }
+  }
+  static __device__ __forceinline__ void fetch(const E* row, int width, int t, const E* begin, const E* end, uint32_t to) {
+#pragma unroll
+    for (int i = 0; i < V * PIECES; ++i) piece(row, width, i * threads() + t, begin, end, to);
+    if (t == 0) piece(row, width, V * PIECES * threads(), begin, end, to);
+  }
+  // octet v of thread t, of which n elements exist, of a row that starts `off` bytes behind its first piece
+  static __device__ __forceinline__ void read(uint32_t from, uint32_t off, int t, int v, int n, Octet<E>& o) {
+    constexpr int WORDS = Octet<E>::WORDS;
+    uint32_t w[WORDS + 7];
+#pragma unroll
+    for (int k = 0; k < PIECES + 1; ++k) {
+      const uint4 q = lds128u(from + uint32_t(((v * threads() + t) * PIECES + k) * 16));
+      w[4 * k] = q.x; w[4 * k + 1] = q.y; w[4 * k + 2] = q.z; w[4 * k + 3] = q.w;
+    }
+    w[WORDS + 4] = w[WORDS + 5] = w[WORDS + 6] = 0u;
+    if constexpr (WORDS == 8) {
+      shift_words<8>(w, off >> 2);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o.q[k] = w[k];
+    } else {
+      shift_words<5>(w, off >> 2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o.q[k] = __funnelshift_r(w[k], w[k + 1], (off & 2u) * 8u);
+    }
+    if (n < 8) o.cut(n);
+  }
+};
+template <bool WARP>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (WARP) __syncwarp();
+  else __syncthreads();
+}
+
 // Bound by HBM (one read, one write), next to it by issue slots.  So few threads with many elements each (a row's two sums cost
-// ten shuffles and a barrier whatever a thread holds), elements widened once, and arithmetic on pairs.  VEC: the next three
-// rows are on their way to shared memory while this one is worked on, each thread copying what it will read.
-template <typename E, bool WARP, int V, bool VEC>
+// ten shuffles and a barrier whatever a thread holds), elements widened once, and arithmetic on pairs.  The next rows are on
+// their way to shared memory while this one is worked on; rows of whole octets that start on 16 bytes are copied by the
+// threads that read them, others (SHIFT) by all and behind a barrier.
+template <typename E, bool WARP, int V, bool SHIFT>
 __global__ void __launch_bounds__(WARP ? 32 * LN_WARP_ROWS : LN_BLOCK, 1)
 ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __restrict__ b, E* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, uint8_t* __restrict__ codes,
                   uint8_t* __restrict__ exponents, int format, long long rows, int width, int groups, float eps) {
-  using Slice = RowSlice<E, WARP, V, VEC>;
+  using Slice = RowSlice<E, WARP, V, !SHIFT>;
+  using Shifted = ShiftedRow<E, WARP, V>;
   constexpr int R = WARP ? LN_WARP_ROWS : 1, SLOT = V * 8 * int(sizeof(E)), STAGES = LN_STAGES<E, WARP, V, 1>;
+  static_assert(STAGES >= 3, "a row fits three times");
   extern __shared__ __align__(16) uint8_t ln_smem[];
   __shared__ float sh[2][LN_MOST_WARPS];
   pdl_wait();
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
   const long long stride = (long long)gridDim.x * R, first = (long long)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
-  // 16-byte pieces of all threads side by side: no bank conflicts
+  // 16-byte pieces of all threads side by side: no bank conflicts; shifted rows: one behind the other
   auto piece = [&](int stage, int k) { return smem_u32(ln_smem) + uint32_t((stage * (SLOT / 16) + k) * blockDim.x + threadIdx.x) * 16u; };
+  auto shifted_at = [&](int stage) { return smem_u32(ln_smem) + (uint32_t(WARP ? threadIdx.x >> 5 : 0) * STAGES + uint32_t(stage)) * Shifted::bytes(); };
   auto fetch = [&](long long row, int stage) {
-    if (VEC && row < rows) {
+    if (row < rows) {
+      if constexpr (SHIFT) {
+        Shifted::fetch(x + row * width, width, t, x, x + rows * width, shifted_at(stage));
+      } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (Slice::inside(t, v, 0, width)) {
-          const E* src = x + row * width + Slice::index(t, v);
+        for (int v = 0; v < V; ++v)
+          if (Slice::inside(t, v, 0, width)) {
+            const E* src = x + row * width + Slice::index(t, v);
 #pragma unroll
-          for (int k = 0; k < int(sizeof(E)) / 2; ++k)
-            copy_async16<E>(piece(stage, v * (int(sizeof(E)) / 2) + k), reinterpret_cast<const uint8_t*>(src) + 16 * k);
-        }
+            for (int k = 0; k < int(sizeof(E)) / 2; ++k)
+              copy_async16<E>(piece(stage, v * (int(sizeof(E)) / 2) + k), reinterpret_cast<const uint8_t*>(src) + 16 * k);
+          }
+      }
     }
     copy_commit();
   };
   Octet<E> wv[V], bv[V];
   const bool scaled = w != nullptr, shifted = b != nullptr;
   const float per_element = 1.f / float(width);
-  if constexpr (VEC) {
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch(first + s * stride, s);
+  for (int s = 0; s < STAGES - 1; ++s) fetch(first + s * stride, s);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (scaled) Slice::load(w, width, t, v, wv[v]);
-      if (shifted) Slice::load(b, width, t, v, bv[v]);
-    }
+  for (int v = 0; v < V; ++v) {
+    if (scaled) Slice::load(w, width, t, v, wv[v]);
+    if (shifted) Slice::load(b, width, t, v, bv[v]);
   }
   int stage = 0;
   for (long long row = first; row < rows; row += stride) {
     Octet<E> in[V];
-    if constexpr (VEC) {
-      static_assert(STAGES >= 3, "a row fits three times");
-      copy_wait<STAGES - 2>();
+    copy_wait<STAGES - 2>();
+    if constexpr (SHIFT) {
+      row_sync<WARP>();
+      const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(x + row * width) & 15u);
+#pragma unroll
+      for (int v = 0; v < V; ++v) Shifted::read(shifted_at(stage), off, t, v, width - Slice::index(t, v), in[v]);
+    } else {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         in[v].clear();
@@ -239,9 +292,6 @@ ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __r
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) Slice::load(x + row * width, width, t, v, in[v], x, x + rows * width);
     }
     unsigned long long xs[V][4], sum = 0ull;
 #pragma unroll
@@ -252,10 +302,9 @@ ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __r
         sum = add2(sum, xs[v][k]);
       }
     const float mean = row_total<WARP>(lane0(sum) + lane1(sum), sh[0]) * per_element;
-    if constexpr (VEC) {          // into the stage of the row before this one: its values have been used
-      fetch(row + (STAGES - 1) * stride, (stage + STAGES - 1) % STAGES);
-      stage = (stage + 1) % STAGES;
-    }
+    // into the stage of the row before this one: its values have been used
+    fetch(row + (STAGES - 1) * stride, (stage + STAGES - 1) % STAGES);
+    stage = (stage + 1) % STAGES;
     sum = 0ull;
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -270,10 +319,6 @@ ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __r
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float u[8], o[8];
-      if constexpr (!VEC) {
-        if (scaled) Slice::load(w, width, t, v, wv[v]);
-        if (shifted) Slice::load(b, width, t, v, bv[v]);
-      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const unsigned long long unit = mul2(xs[v][k], both(rstd));
@@ -332,10 +377,10 @@ ln_dx_loop_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __restr
 }
 
 // The end of a backward kernel: a block's sums over its rows leave as one line of partials (bands, 2, width).
-template <typename E, bool WARP, int V, bool VEC>
+template <typename E, bool WARP, int V>
 __device__ __forceinline__ void store_row_sums(const unsigned long long (&dw)[V][4], const unsigned long long (&db)[V][4], float* partials,
                                                int width) {
-  using Slice = RowSlice<E, WARP, V, VEC>;
+  using Slice = RowSlice<E, WARP, V, true>;
   constexpr int R = WARP ? LN_WARP_ROWS : 1;
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
   if (partials == nullptr) return;
@@ -372,91 +417,16 @@ __device__ __forceinline__ void store_row_sums(const unsigned long long (&dw)[V]
 }
 
 // Rows in registers: one read of dy and of what was kept serves dx and both sums over rows.  A thread keeps the same columns
-// for all rows of its block (blockIdx.x, blockIdx.x + gridDim.x, ...) and adds them up in registers.  This kernel takes rows that
-// start anywhere.
-template <typename E, bool WARP, int V>
-__global__ void __launch_bounds__(WARP ? 32 * LN_WARP_ROWS : LN_BLOCK)
-ln_backward_any_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __restrict__ rstd_in, const E* __restrict__ w,
-                       E* __restrict__ dx, float* __restrict__ partials, int format, long long rows, int width) {
-  using Slice = RowSlice<E, WARP, V, false>;
-  constexpr int R = WARP ? LN_WARP_ROWS : 1;
-  __shared__ float sh[2][2 * LN_MOST_WARPS];
-  clear_totals(sh);
-  pdl_wait();
-  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const long long stride = (long long)gridDim.x * R;
-  unsigned long long dw[V][4], db[V][4];
-#pragma unroll
-  for (int v = 0; v < V; ++v)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) dw[v][k] = db[v][k] = 0ull;
-  const float per_element = 1.f / float(width);
-  int turn = 0;
-  for (long long row = (long long)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0); row < rows; row += stride, turn ^= 1) {
-    Octet<E> in[V], raw[V];
-    const float rstd = rstd_in[row], mean = format < 0 ? kept.mean[row] : 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      Slice::load(dy + row * width, width, t, v, in[v], dy, dy + rows * width);
-      if (format < 0) Slice::load(kept.x + row * width, width, t, v, raw[v], kept.x, kept.x + rows * width);
-      else Slice::load_eight(kept.codes + row * kept.groups * EIGHT_GROUP, kept.exponents + row * kept.groups, width, t, v, raw[v]);
-    }
-    // u = the normalised row, g = dy w of octet v; behind the width dy is zero
-    auto octet = [&](int v, unsigned long long (&u)[4], unsigned long long (&g)[4]) {
-      if (format < 0) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = mul2(add2(raw[v].get(k), both(-mean)), both(rstd));
-      } else {
-        float f[8];
-        if (format == EIGHT_INT8) Slice::template get_eight<EIGHT_INT8>(raw[v], f);
-        else Slice::template get_eight<EIGHT_E4M3>(raw[v], f);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = pair(f[2 * k], f[2 * k + 1]);
-      }
-      Octet<E> wv;
-      if (w != nullptr) Slice::load(w, width, t, v, wv);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) g[k] = w != nullptr ? mul2(in[v].get(k), wv.get(k)) : in[v].get(k);
-    };
-    unsigned long long sg = 0ull, su = 0ull;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      unsigned long long u[4], g[4];
-      octet(v, u, g);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        dw[v][k] = fma2(in[v].get(k), u[k], dw[v][k]);
-        db[v][k] = add2(db[v][k], in[v].get(k));
-        sg = add2(sg, g[k]);
-        su = fma2(g[k], u[k], su);
-      }
-    }
-    if (dx == nullptr) continue;                  // uniform over the grid
-    const float2 s = row_total<WARP>(make_float2(lane0(sg) + lane1(sg), lane0(su) + lane1(su)), sh[turn]);
-    const unsigned long long mg = both(-s.x * per_element), mu = both(-s.y * per_element);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      unsigned long long u[4], g[4];
-      float o[8];
-      octet(v, u, g);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const unsigned long long q = mul2(fma2(mu, u[k], add2(g[k], mg)), both(rstd));
-        o[2 * k] = lane0(q); o[2 * k + 1] = lane1(q);
-      }
-      Slice::store(dx + row * width, width, t, v, o);
-    }
-  }
-  store_row_sums<E, WARP, V, false>(dw, db, partials, width);
-}
-
-// The same for rows that start on 16 bytes.  Bound by issue slots and HBM alike (at 16384 rows of 4096 BF16 a first version with
+// for all rows of its block (blockIdx.x, blockIdx.x + gridDim.x, ...) and adds them up in registers.
+//
+// Bound by issue slots and HBM alike (at 16384 rows of 4096 BF16 a first version with
 // scalar arithmetic issued 34 instructions per 32 elements' worth of work, 2.6 a cycle).  Hence: arithmetic on pairs, two sums
 // for the price of one exchange, pointers that advance instead of row * width, and a ring of rows in shared memory that each
 // thread fills for itself with asynchronous copies, 16-byte pieces of all threads side by side (with a thread's pieces
 // together, 272 bytes from its neighbour's, a pass took 109 us instead of 81).
+// SHIFT: rows that start anywhere, their pieces copied by all threads of the row and read behind a barrier.
 // V <= 2 keeps u and g in registers between the two sweeps; V = 4 (rows above 8192) reads them again from shared memory.
-template <typename E, bool WARP, int V, int FORMAT>
+template <typename E, bool WARP, int V, int FORMAT, bool SHIFT>
 __global__ void __launch_bounds__(WARP ? 32 * LN_WARP_ROWS : LN_BLOCK)
 ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __restrict__ rstd_in, const E* __restrict__ w,
                    E* __restrict__ dx, float* __restrict__ partials, long long rows, int width) {
@@ -464,6 +434,7 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
   constexpr int STAGES = LN_STAGES<E, WARP, V, 2>;                          // 1: a row is fetched when its turn comes
   constexpr int STAGE_PIECES = 2 * V * PIECES;
   constexpr bool HOLD = V <= 2;
+  using Shifted = ShiftedRow<E, WARP, V>;
   extern __shared__ __align__(16) uint8_t ln_smem[];
   __shared__ float sh[2][2 * LN_MOST_WARPS];
   clear_totals(sh);
@@ -471,23 +442,36 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
   const int t = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : int(blockDim.x);
   const long long stride = (long long)gridDim.x * R, first = (long long)blockIdx.x * R + (WARP ? threadIdx.x >> 5 : 0);
   const long long count = first < rows ? (rows - first + stride - 1) / stride : 0;
-  const uint32_t mine = smem_u32(ln_smem) + uint32_t(threadIdx.x) * 16u, apart = uint32_t(blockDim.x) * 16u;
+  // stages are `stage_bytes` apart from `mine` on: pieces of all threads side by side, or (SHIFT) a row's two inputs in order
+  const uint32_t apart = uint32_t(blockDim.x) * 16u, stage_bytes = SHIFT ? 2u * Shifted::bytes() : uint32_t(STAGE_PIECES) * apart;
+  const uint32_t mine = smem_u32(ln_smem) + (SHIFT ? uint32_t(WARP ? threadIdx.x >> 5 : 0) * uint32_t(STAGES) * stage_bytes : uint32_t(threadIdx.x) * 16u);
   bool inside[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) inside[v] = 8 * (v * threads + t) < width;
 
   // what is fetched next: pointers to this thread's first octet of the row, and how many rows are left to fetch
   const long long step = stride * width;
-  const E* next_dy = dy + first * width + 8 * t;
-  const E* next_x = FORMAT < 0 ? kept.x + first * width + 8 * t : nullptr;
+  const E* next_dy = dy + first * width + (SHIFT ? 0 : 8 * t);
+  const E* next_x = FORMAT < 0 ? kept.x + first * width + (SHIFT ? 0 : 8 * t) : nullptr;
+  // bytes by which this row and its kept row start behind a piece, and what they gain from row to row
+  uint32_t off_dy = uint32_t(reinterpret_cast<uintptr_t>(next_dy) & 15u), off_x = FORMAT < 0 ? uint32_t(reinterpret_cast<uintptr_t>(next_x) & 15u) : 0u;
+  const uint32_t off_step = uint32_t((unsigned long long)step * sizeof(E)) & 15u;
   const long long code_step = stride * kept.groups * EIGHT_GROUP, byte_step = stride * kept.groups;
   const uint8_t* next_codes = FORMAT >= 0 ? kept.codes + first * kept.groups * EIGHT_GROUP + 8 * t : nullptr;
   long long to_fetch = count;
   auto fetch = [&](uint32_t at) {
     if (to_fetch > 0) {
+      if constexpr (SHIFT) {
+        Shifted::fetch(next_dy, width, t, dy, dy + rows * width, at);
+        if constexpr (FORMAT < 0) Shifted::fetch(next_x, width, t, kept.x, kept.x + rows * width, at + Shifted::bytes());
+      }
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (!inside[v]) continue;
+        if constexpr (SHIFT) {
+          if (FORMAT >= 0) copy_async8(at + Shifted::bytes() + uint32_t(v * threads + t) * 8u, next_codes + 8 * v * threads);
+          continue;
+        }
 #pragma unroll
         for (int k = 0; k < PIECES; ++k) {
           copy_async16<E>(at + uint32_t(v * PIECES + k) * apart, reinterpret_cast<const uint8_t*>(next_dy + 8 * v * threads) + 16 * k);
@@ -526,23 +510,28 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
   const float per_element = 1.f / float(width);
   const bool scaled = w != nullptr;
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) fetch(mine + uint32_t(s * STAGE_PIECES) * apart);
+  for (int s = 0; s < STAGES - 1; ++s) fetch(mine + uint32_t(s) * stage_bytes);
   Octet<E> wv[V];
   auto load_w = [&](int v) {
     wv[v].clear();
-    if (inside[v]) wv[v].load(w + 8 * (v * threads + t));
+    if constexpr (SHIFT) load_any<E>(wv[v], w + 8 * (v * threads + t), width - 8 * (v * threads + t), w, w + width);
+    else if (inside[v]) wv[v].load(w + 8 * (v * threads + t));
   };
   if (HOLD && scaled) {
 #pragma unroll
     for (int v = 0; v < V; ++v) load_w(v);
   }
   if (count > 0) fetch_small();
-  uint32_t at = 0, refill = uint32_t((STAGES - 1) * STAGE_PIECES) * apart;    // offsets of this row's stage and of the free one
+  uint32_t at = 0, refill = uint32_t(STAGES - 1) * stage_bytes;    // offsets of this row's stage and of the free one
   E* out = dx != nullptr ? dx + first * width + 8 * t : nullptr;
   int turn = 0;
   for (long long i = 0; i < count; ++i) {
-    if (STAGES == 1) fetch(mine);
+    if (STAGES == 1) {
+      if (SHIFT) row_sync<WARP>();              // the only stage has been read by all
+      fetch(mine);
+    }
     copy_wait<STAGES == 1 ? 0 : STAGES - 2>();
+    if (SHIFT) row_sync<WARP>();
     const float mean = next_mean, rstd = next_rstd;
     uint32_t byte[V];
 #pragma unroll
@@ -552,7 +541,16 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
       Octet<E> raw;
       d.clear();
       raw.clear();
-      if (inside[v]) {
+      if constexpr (SHIFT) {
+        const int n = width - 8 * (v * threads + t);
+        Shifted::read(mine + at, off_dy, t, v, n, d);
+        if constexpr (FORMAT < 0) {
+          Shifted::read(mine + at + Shifted::bytes(), off_x, t, v, n, raw);
+        } else if (inside[v]) {
+          const uint32_t c = mine + at + Shifted::bytes() + uint32_t(v * threads + t) * 8u;
+          raw.q[0] = lds32u(c); raw.q[1] = lds32u(c + 4u);
+        }
+      } else if (inside[v]) {
 #pragma unroll
         for (int k = 0; k < PIECES; ++k) {
           const uint4 q = lds128u(mine + at + uint32_t(v * PIECES + k) * apart);
@@ -606,7 +604,13 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
           const unsigned long long q = mul2(fma2(mu, u[k], add2(g[k], mg)), both(rstd));
           o[2 * k] = lane0(q); o[2 * k + 1] = lane1(q);
         }
-        if (inside[v]) store8<E>(out + 8 * v * threads, o);
+        if constexpr (SHIFT) {
+          Octet<E> packed;
+          packed.pack(o);
+          store_any<E>(out + 8 * v * threads, min(8, max(0, width - 8 * (v * threads + t))), packed);
+        } else if (inside[v]) {
+          store8<E>(out + 8 * v * threads, o);
+        }
       }
       out += step;
     }
@@ -614,11 +618,13 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
     if (STAGES > 1) {
       fetch(mine + refill);
       refill = at;
-      at += uint32_t(STAGE_PIECES) * apart;
-      if (at == uint32_t(STAGES * STAGE_PIECES) * apart) at = 0;
+      at += stage_bytes;
+      if (at == uint32_t(STAGES) * stage_bytes) at = 0;
     }
+    off_dy = (off_dy + off_step) & 15u;
+    off_x = (off_x + off_step) & 15u;
   }
-  store_row_sums<E, WARP, V, true>(dw, db, partials, width);
+  store_row_sums<E, WARP, V>(dw, db, partials, width);
 }
 
 // ---- wider rows: the sums over rows apart, see store_column_sums
