@@ -18,6 +18,15 @@ unsigned octet_blocks(long long octets) {
   const long long blocks = (octets + EIGHT_THREADS * EIGHT_UNROLL - 1) / (EIGHT_THREADS * EIGHT_UNROLL);
   return blocks <= 0x7fffffffLL ? unsigned(blocks) : 0;
 }
+// 16-bit rows of whole octets on 16 bytes take a kernel of their own (the workspace of a linear layer's backward pass).
+template <typename Out, int FORMAT>
+auto restore_rows(const void* out, int pitch) {
+  auto kernel = eight_restore_rows_kernel<Out, FORMAT, false>;
+  if constexpr (sizeof(Out) == 2) {
+    if (pitch % 8 == 0 && on_octets(out, 2)) kernel = eight_restore_rows_kernel<Out, FORMAT, true>;
+  }
+  return kernel;
+}
 dim3 row_blocks(long long rows, int groups) {
   const unsigned segments = unsigned(cdiv(groups, EIGHT_SEGMENT));
   const long long most = std::max<long long>(1, 148LL * 32 / segments);
@@ -56,13 +65,8 @@ int eight_restore(const void* codes, const void* exponents, long long rows, int 
       auto kernel = format == EIGHT_INT8 ? eight_restore_octets_kernel<Out, EIGHT_INT8> : eight_restore_octets_kernel<Out, EIGHT_E4M3>;
       launch(kernel, octet_blocks(octets), EIGHT_THREADS, 0, stream, c, e, to, octets);
     } else {
-      DISPATCH_FORMAT(format, F, {
-        auto kernel = eight_restore_rows_kernel<Out, F < 0 ? EIGHT_INT8 : F, false>;
-        if constexpr (sizeof(Out) == 2) {
-          if (pitch % 8 == 0 && on_octets(out, 2)) kernel = eight_restore_rows_kernel<Out, F < 0 ? EIGHT_INT8 : F, true>;
-        }
-        launch(kernel, row_blocks(rows, groups), EIGHT_THREADS, 0, stream, c, e, to, rows, width, groups, pitch);
-      });
+      auto kernel = format == EIGHT_INT8 ? restore_rows<Out, EIGHT_INT8>(out, pitch) : restore_rows<Out, EIGHT_E4M3>(out, pitch);
+      launch(kernel, row_blocks(rows, groups), EIGHT_THREADS, 0, stream, c, e, to, rows, width, groups, pitch);
     }
   });
   LAUNCH_CHECK("activation_restore");

@@ -30,11 +30,17 @@ struct LnFamily {
 };
 template <int MOST, class F>
 void with_ln_shape(const LnShape& s, F&& f) {
-  if (s.threads == 32 && s.octets == 1) f(LnFamily<true, 1>{});
-  else if (s.threads == 32 && s.octets == 2) f(LnFamily<true, 2>{});
-  else if (MOST == 4 && s.threads == 32) f(LnFamily<true, MOST>{});
-  else if (MOST == 2 && s.octets == 2) f(LnFamily<false, MOST>{});
-  else f(LnFamily<false, 4>{});
+  const bool warp = s.threads == 32;
+  if (warp && s.octets == 1) return f(LnFamily<true, 1>{});
+  if (warp && s.octets == 2) return f(LnFamily<true, 2>{});
+  if constexpr (MOST == 4) {
+    if (warp && s.octets == 3) return f(LnFamily<true, 3>{});
+    if (warp) return f(LnFamily<true, 4>{});
+    if (s.octets == 3) return f(LnFamily<false, 3>{});
+  } else {
+    if (s.octets == 2) return f(LnFamily<false, 2>{});
+  }
+  f(LnFamily<false, 4>{});
 }
 // Rows that start on 16 bytes throughout.
 bool ln_vectors(int width, std::initializer_list<const void*> tensors) {

@@ -228,7 +228,7 @@ __device__ __forceinline__ void row_sync() {
 // their way to shared memory while this one is worked on; rows of whole octets that start on 16 bytes are copied by the
 // threads that read them, others (SHIFT) by all and behind a barrier.
 template <typename E, bool WARP, int V, bool SHIFT>
-__global__ void __launch_bounds__(WARP ? 32 * LN_WARP_ROWS : LN_BLOCK, 1)
+__global__ void __launch_bounds__(WARP ? 32 * LN_WARP_ROWS : LN_BLOCK, WARP ? 4 : 1)       // 512 threads per SM
 ln_forward_kernel(const E* __restrict__ x, const E* __restrict__ w, const E* __restrict__ b, E* __restrict__ y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, uint8_t* __restrict__ codes,
                   uint8_t* __restrict__ exponents, int format, long long rows, int width, int groups, float eps) {
@@ -470,14 +470,14 @@ ln_backward_kernel(const E* __restrict__ dy, LnKept<E> kept, const float* __rest
         if (!inside[v]) continue;
         if constexpr (SHIFT) {
           if (FORMAT >= 0) copy_async8(at + Shifted::bytes() + uint32_t(v * threads + t) * 8u, next_codes + 8 * v * threads);
-          continue;
-        }
+        } else {
 #pragma unroll
-        for (int k = 0; k < PIECES; ++k) {
-          copy_async16<E>(at + uint32_t(v * PIECES + k) * apart, reinterpret_cast<const uint8_t*>(next_dy + 8 * v * threads) + 16 * k);
-          if (FORMAT < 0) copy_async16<E>(at + uint32_t((V + v) * PIECES + k) * apart, reinterpret_cast<const uint8_t*>(next_x + 8 * v * threads) + 16 * k);
+          for (int k = 0; k < PIECES; ++k) {
+            copy_async16<E>(at + uint32_t(v * PIECES + k) * apart, reinterpret_cast<const uint8_t*>(next_dy + 8 * v * threads) + 16 * k);
+            if (FORMAT < 0) copy_async16<E>(at + uint32_t((V + v) * PIECES + k) * apart, reinterpret_cast<const uint8_t*>(next_x + 8 * v * threads) + 16 * k);
+          }
+          if (FORMAT >= 0) copy_async8(at + uint32_t((V + v) * PIECES) * apart, next_codes + 8 * v * threads);
         }
-        if (FORMAT >= 0) copy_async8(at + uint32_t((V + v) * PIECES) * apart, next_codes + 8 * v * threads);
       }
       next_dy += step;
       if (FORMAT < 0) next_x += step;

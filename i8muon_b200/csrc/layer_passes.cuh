@@ -258,7 +258,7 @@ linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict_
       for (long long row = first + warp; row < last; row += DZ_WARPS * DZ_ROWS) {
         Octet<E> d[DZ_ROWS];
         uint4 z[DZ_ROWS];
-        uint32_t byte[DZ_ROWS];
+        [[maybe_unused]] uint32_t byte[DZ_ROWS];
 #pragma unroll
         for (int r = 0; r < DZ_ROWS; ++r) {
           const long long at = row + r * DZ_WARPS;

@@ -43,10 +43,12 @@ struct LnShape {
 };
 inline LnShape ln_shape(int width, int most) {
   const int octets = width / 8 + (width % 8 != 0);
-  for (int v = 1; v <= most; v *= 2)
-    if (octets <= 32 * v) return {32, v};
+  if (octets <= 32 * most) return {32, most == 2 && octets > 32 ? 2 : (octets + 31) / 32};
+  // whole warps of threads; three octets instead of four where that leaves fewer idle (forward)
+  auto threads = [&](int v) { return ((octets + v - 1) / v + 31) / 32 * 32; };
+  if (most == 4 && threads(3) <= 512 && threads(3) * 3 < threads(4) * 4) return {threads(3), 3};
   for (int v = most; v <= 4; v *= 2)
-    if (octets <= 512 * v) return {((octets + v - 1) / v + 31) / 32 * 32, v};
+    if (threads(v) <= 512) return {threads(v), v};
   return {0, 0};
 }
 // Bands of the backward pass's sums over rows, one per block of the register kernels: 512 resident threads per SM.

@@ -103,7 +103,10 @@ def _status(device) -> int:
 
 
 def _any_gradient(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 # ------------------------------------------------------- activations in eight bits
