@@ -77,9 +77,18 @@ int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int ex
   cuuint64_t strides[2] = {cuuint64_t(pitch) * esize, cuuint64_t(pitch) * esize * rows};
   cuuint32_t box[3] = {cuuint32_t(128 / esize), cuuint32_t(mn ? 128 / esize : box_rows), 1u};
   cuuint32_t estr[3] = {1u, 1u, 1u};
-  CUresult r = g_encode(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return g_encode(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {   // the first CUDA work of this thread: no runtime call has made a context current yet
+    int device;
+    CUDA_TRY(cudaGetDevice(&device));
+    CUDA_TRY(cudaSetDevice(device));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) return fail(I8M_E_CUDA, "cuTensorMapEncodeTiled failed with code %d", int(r));
   return 0;
 }

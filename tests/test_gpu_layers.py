@@ -1,5 +1,8 @@
 """The layer operators against their formulas in 64 bits (layer_reference.py), through the public entry points."""
 import math
+import pathlib
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -585,3 +588,33 @@ def test_a_first_call_on_a_device_is_not_captured(cuda_device, monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="before capturing"):
         linear(x, w)
+
+
+FRESH_THREADS = """
+import threading
+import torch
+from i8muon_b200 import check_status, linear
+x, w = (torch.full(s, 0.125, dtype=torch.bfloat16, device="cuda", requires_grad=True) for s in ((128, 256), (192, 256)))
+dy = torch.ones(128, 192, dtype=torch.bfloat16, device="cuda")
+spare = [torch.empty(1 << 16, device="cuda") for _ in range(8)]   # what the threads allocate is there already
+y = linear(x, w)
+del spare
+dx, dw = torch.autograd.grad(y, (x, w), dy)        # the first work of autograd's thread of this device
+assert (dx == 24).all() and (dw == 16).all() and (y == 4).all()
+seen = []
+def forward():
+    seen.append(linear(x.detach(), w.detach()))    # the first work of a thread of the user's
+thread = threading.Thread(target=forward)
+thread.start()
+thread.join()
+torch.cuda.synchronize()
+assert len(seen) == 1 and torch.equal(seen[0], y)
+check_status()
+"""
+
+
+def test_the_first_work_of_a_thread(cuda_device):
+    """A new thread has no current context before its first runtime call: a child process, for threads that are new."""
+    root = pathlib.Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", FRESH_THREADS], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
