@@ -88,7 +88,9 @@ __device__ __forceinline__ unsigned long long derivative(unsigned long long z) {
     return fma2(mul2(b, both(0.39894228040143268f)), n.density, pair(z0 < 0.f ? t0 : 1.f - t0, z1 < 0.f ? t1 : 1.f - t1));
   }
   if constexpr (ACT == ACT_GELU_TANH) {
-    const unsigned long long q = mul2(z, z), s = gate2(mul2(z, fma2(both(-LOG2_E * GELU_TANH_K), q, both(-LOG2_E * GELU_TANH_C))));
+    // z^2 bounded, so that the slope is finite where s (1 - s) is zero (from |z| = 10 on); a NaN stays one in z itself
+    const unsigned long long q = pair(fminf(z0 * z0, 1e30f), fminf(z1 * z1, 1e30f));
+    const unsigned long long s = gate2(mul2(z, fma2(both(-LOG2_E * GELU_TANH_K), q, both(-LOG2_E * GELU_TANH_C))));
     const unsigned long long slope = fma2(both(3.f * GELU_TANH_K), q, both(GELU_TANH_C));
     return fma2(mul2(mul2(z, s), fma2(s, both(-1.f), both(1.f))), slope, s);
   }

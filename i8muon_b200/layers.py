@@ -392,7 +392,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     gradient of the pre-activation is rounded to the type of ``x`` once, as the operand of the two backward products.
 
     A device-side wait that runs out is reported through the status word that ``check_status()`` and ``Muon.step()`` read; a
-    first call on a device cannot be captured into a graph."""
+    first call on a device cannot be captured into a graph.  A backward pass is captured together with its forward pass, on
+    one stream, when no graph of the same leaves is alive that was built on another stream (autograd would join that stream)."""
     fmt = _format(checkpoint, "linear")
     if activation is not None and not isinstance(activation, str) or activation not in _ACTIVATIONS:
         raise ValueError("linear: activation must be None, 'relu', 'relu2', 'gelu', 'gelu_tanh' or 'silu'")

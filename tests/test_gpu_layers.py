@@ -341,6 +341,22 @@ def test_linear_gradients_against_differences(cuda_device):
                 assert abs((side[0] - side[1]) / 2e-4 - got[k].reshape(-1)[i].item()) < 2.0 ** -11 * 3 * 4 * 4
 
 
+@pytest.mark.parametrize("act", ["relu", "relu2", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dtype, z", [(torch.float16, 6e4), (torch.bfloat16, 6e4), (torch.bfloat16, 1e20), (torch.bfloat16, 3e38)])
+def test_derivatives_far_out(cuda_device, act, dtype, z):
+    """z is the bias alone.  The slopes there are 1 and 0 to the last bit, and 2 z for relu2 (rounded once: half a step)."""
+    bias = torch.tensor([z, -z] * 8, dtype=dtype, device=cuda_device).requires_grad_()
+    x, w = (torch.zeros(s, dtype=dtype, device=cuda_device) for s in ((1, 64), (16, 64)))
+    y = linear(x, w, bias, activation=act)
+    got, = torch.autograd.grad(y, bias, torch.ones_like(y))
+    slope = 2 * bias.detach().double() if act == "relu2" else torch.ones(16, dtype=torch.float64, device=cuda_device)
+    want = torch.where(bias > 0, slope, 0.0).to(dtype)
+    assert torch.equal(got, want)
+    top = bias.detach().double() ** (2 if act == "relu2" else 1)
+    assert torch.equal(y[0].detach(), torch.where(bias > 0, top, 0.0).to(dtype))
+    check_status()
+
+
 def test_linear_edges(cuda_device):
     dtype = torch.bfloat16
     w, b = normal((8, 16), 1, dtype, cuda_device).requires_grad_(), normal((8,), 2, dtype, cuda_device).requires_grad_()
