@@ -22,7 +22,8 @@ struct Operand {
 struct Plan {
   int bn, split;
 };
-// The least of an estimate in nanoseconds.  Pairs: 6 us, and 0.365 us per K block of a wave of units.  Split kernel: 4.5 us and 25 ns
+// The least of an estimate in nanoseconds.  Pairs: 6 us, and 0.365 us per K block of a wave of units, at least 1.85 us (an epilogue)
+// for every wave but the first.  Split kernel: 4.5 us and 25 ns
 // per column of the tile for its start, sums and end, 4 us for every further wave, and per K block 14 ns for each KB that the
 // CTA takes in, at least 0.27 us, or 17 ns per KB where two CTAs share an SM.  Both: beside the time that DRAM takes for the
 // operands (as the root of the sum of squares: neither hides the other fully).
@@ -36,7 +37,7 @@ Plan plan_product(int rows, int features, int k, bool rows_mn, int sms) {
   auto beside_dram = [&](double v) { return std::sqrt(v * v + dram * dram); };
   const long long units = (long long)cdiv(rows, 2 * TILE) * cdiv(features, 2 * TILE), pairs = std::max(1, sms / 2);
   Plan best{0, 1};
-  double cost = 6000 + beside_dram((units + pairs - 1) / pairs * num_kb * 365.0);
+  double cost = 6000 + beside_dram(num_kb * 365.0 + ((units + pairs - 1) / pairs - 1) * std::max(1850.0, num_kb * 365.0));
   for (int bn = rows_mn ? 64 : 16; bn <= 128; bn *= 2) {
     const long long split_tiles = (long long)cdiv(features, TILE) * cdiv(rows, bn), kilobytes = 16 + bn / 8;
     for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
@@ -90,13 +91,22 @@ int product_split(const Plan& plan, const Operand& a, const Operand& b, int m, i
   }
 }
 
+// Rows of `width` 16-bit elements, one behind the other, that tensor copies can address.
+bool addressable(const void* p, int width) { return width % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 template <typename E, int A_MN, int B_MN>
-int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g, const LinearArgs& args, unsigned pairs,
+int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g, LinearArgs args, unsigned pairs,
                 cudaStream_t stream, const char* name) {
+  CUtensorMap my = ma, mz = ma;          // what is not stored through its map has none
+  args.y_blocks = addressable(args.y, g.n);
+  if (args.y_blocks)
+    if (int rc = make_block_map(&my, args.y, g.n, g.m, g.n)) return rc;
+  if (args.z != nullptr)
+    if (int rc = make_block_map(&mz, args.z, args.z_pitch, g.m, args.z_pitch)) return rc;
   auto kernel = linear_pair_kernel<E, A_MN, B_MN>;
   static SmemAllowed allowed;
   if (int rc = allow_smem(allowed, kernel, LPR_SMEM)) return rc;
-  launch_clusters(kernel, 2, 2 * pairs, LPR_THREADS, LPR_SMEM, stream, ma, mb, g, args);
+  launch_clusters(kernel, 2, 2 * pairs, LPR_THREADS, LPR_SMEM, stream, ma, mb, my, mz, g, args);
   LAUNCH_CHECK(name);
   return 0;
 }
@@ -131,8 +141,6 @@ template <typename... A>
 int product_of(int dtype, A&&... args) {
   return dtype == I8M_F16 ? product<__half>(std::forward<A>(args)...) : product<__nv_bfloat16>(std::forward<A>(args)...);
 }
-
-bool addressable(const void* p, int width) { return width % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_linear(const char* name, int rows, int inner, int outer, int dtype, int activation, int format) {
   if (rows < 1 || inner < 1 || outer < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);

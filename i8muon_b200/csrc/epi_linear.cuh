@@ -3,6 +3,11 @@
 // in FP32, rounded once.  In training the pre-activation z leaves beside y for the backward pass, rounded to the operand
 // type or in eight bits: a thread holds 32 columns of one row, which is a group of that format, so its exponent needs no
 // exchange.  The two backward products run through the same epilogue with nothing but y.
+//
+// What bounds it is instruction issue, not the stores: without them a product with K = 64 took 65 us instead of 68, without
+// anything behind the accumulator 35.  Hence one switch over the activations around a warp's blocks, blocks that leave
+// as tensor copies (one request of one lane, clipped by the copy engine, instead of four loads and stores per lane with
+// their predicates), and a residual that is on its way to L2 while the unit before it is finished.
 #pragma once
 #include "activations.cuh"
 #include "eight_bit.cuh"
@@ -17,6 +22,7 @@ struct LinearArgs {
   uint8_t* codes;          // or in eight bits: (lm, 32 groups), (lm, groups), or NULL
   uint8_t* exponents;
   int z_pitch, groups, format, activation;
+  int y_blocks;            // rows of y start on 16 bytes: blocks leave as tensor copies
 };
 
 __device__ __forceinline__ bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -69,18 +75,49 @@ struct EpiLinear {
   static constexpr uint32_t IDESC = make_idesc(1u, FMT, FMT, TILE, TILE);
   using Args = LinearArgs;
 
-  template <class Acc>
-  static __device__ __forceinline__ void run(const GemmGeom& g, const Args& a, const TileCtx& t, const Acc& acc) {
+  // A 32 x 32 block held one row per lane leaves as one tensor copy (a box of 32 rows of 64 bytes, swizzled within 512 bytes),
+  // clipped to the tensor.  The copy reads the patch after this returns: patch_free before its next use.
+  static __device__ __forceinline__ void patch_free(const WarpPatch& wp) {
+    if (wp.lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+  }
+  static __device__ __forceinline__ void store_block(const WarpPatch& wp, const CUtensorMap* map, int col, int row, const uint32_t (&p)[16]) {
+    patch_free(wp);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      sts128u(wp.base + uint32_t(wp.lane * 64 + ((i ^ (wp.lane >> 1)) & 3) * 16), make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]));
+    fence_proxy_async();
+    __syncwarp();
+    if (wp.lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                   "r"(wp.base), "r"(col), "r"(row), "r"(0)
+                   : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+
+  // Brings the residual's row `row` of a warp's 64 columns from `col` on into L2: called a unit ahead of its use.
+  static __device__ __forceinline__ void expect_residual(const GemmGeom& g, const Args& a, int row, int col) {
+    if (a.residual == nullptr || row >= g.lm || col >= g.ln) return;
+    const E* r = static_cast<const E*>(a.residual) + size_t(row) * g.ln;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(r + col));
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(r + min(col + 63, g.ln - 1)));
+  }
+
+  // This warp's blocks of the tile.
+  template <int ACT, class Acc>
+  static __device__ __forceinline__ void blocks(const GemmGeom& g, const Args& a, const CUtensorMap* map_y, const CUtensorMap* map_z,
+                                                const TileCtx& t, const Acc& acc) {
     const WarpPatch wp{smem_u32(t.wsm), t.lane};
     const int wrow0 = t.row0 + 32 * t.q;
-    const bool vectors = (g.ln & 7) == 0;      // rows of y and of the residual start on 16 bytes with their tensors
+    const bool residual_vectors = a.residual != nullptr && (g.ln & 7) == 0 && on_16_bytes(a.residual);
 #pragma unroll 1
     for (int c = t.c_begin; c < t.c_end; ++c) {
-      uint32_t v[32];
-      acc.load(c, v);
       const int colb = t.col0 + c * 32;
       if (colb >= g.ln || wrow0 >= g.lm) continue;               // uniform over the warp
       const BlockClip clip{g.lm - wrow0, g.ln - colb};
+      uint32_t v[32];
+      acc.load(c, v);
       unsigned long long z[16];
 #pragma unroll
       for (int k = 0; k < 16; ++k) z[k] = pack2(v[2 * k], v[2 * k + 1]);
@@ -103,26 +140,19 @@ struct EpiLinear {
       uint32_t p[16];
       if (a.z != nullptr) {
         pack_row<E>(z, p);
-        wp.write_own_row(p);
-        __syncwarp();
-        store_block_rows(wp, reinterpret_cast<uint8_t*>(static_cast<E*>(a.z) + size_t(wrow0) * a.z_pitch + colb),
-                         size_t(a.z_pitch) * 2, clip.rows, (a.z_pitch - colb) * 2);
-        __syncwarp();
+        store_block(wp, map_z, colb, wrow0, p);
       }
       if (a.codes != nullptr && t.row < g.lm) {
         const size_t group = size_t(t.row) * a.groups + (colb >> 5);
         if (a.format == EIGHT_INT8) store_group<EIGHT_INT8>(z, a.codes + group * 32, a.exponents + group);
         else store_group<EIGHT_E4M3>(z, a.codes + group * 32, a.exponents + group);
       }
-      __syncwarp();
-      with_activation(a.activation, [&](auto act) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) z[k] = activate<decltype(act)::value>(z[k]);
-      });
-      const size_t first = size_t(wrow0) * g.ln + colb;
+      for (int k = 0; k < 16; ++k) z[k] = activate<ACT>(z[k]);
       if (a.residual != nullptr) {
-        const E* r = static_cast<const E*>(a.residual) + first;
-        if (vectors && on_16_bytes(a.residual)) load_block_rows(wp, reinterpret_cast<const uint8_t*>(r), size_t(g.ln) * 2, clip.rows, clip.cols * 2);
+        patch_free(wp);
+        const E* r = static_cast<const E*>(a.residual) + size_t(wrow0) * g.ln + colb;
+        if (residual_vectors) load_block_rows(wp, reinterpret_cast<const uint8_t*>(r), size_t(g.ln) * 2, clip.rows, clip.cols * 2);
         else load_block_elements16(wp, reinterpret_cast<const uint16_t*>(r), size_t(g.ln), clip.rows, clip.cols);
         __syncwarp();
         wp.read_own_row(p);
@@ -131,13 +161,21 @@ struct EpiLinear {
         for (int k = 0; k < 16; ++k) z[k] = add2(z[k], widen2<E>(p[k]));
       }
       pack_row<E>(z, p);
-      wp.write_own_row(p);
-      __syncwarp();
-      E* y = static_cast<E*>(a.y) + first;
-      if (vectors && on_16_bytes(a.y)) store_block_rows(wp, reinterpret_cast<uint8_t*>(y), size_t(g.ln) * 2, clip.rows, clip.cols * 2);
-      else store_block_elements16(wp, reinterpret_cast<uint16_t*>(y), size_t(g.ln), clip.rows, clip.cols);
-      __syncwarp();                            // the patch is free for the next chunk
+      if (a.y_blocks) {
+        store_block(wp, map_y, colb, wrow0, p);
+      } else {
+        patch_free(wp);
+        wp.write_own_row(p);
+        __syncwarp();
+        store_block_elements16(wp, reinterpret_cast<uint16_t*>(a.y) + size_t(wrow0) * g.ln + colb, size_t(g.ln), clip.rows, clip.cols);
+        __syncwarp();
+      }
     }
+  }
+  template <class Acc>
+  static __device__ __forceinline__ void run(const GemmGeom& g, const Args& a, const CUtensorMap* map_y, const CUtensorMap* map_z,
+                                             const TileCtx& t, const Acc& acc) {
+    with_activation(a.activation, [&](auto act) { blocks<decltype(act)::value>(g, a, map_y, map_z, t, acc); });
   }
 };
 

@@ -13,8 +13,10 @@
 //   warp 0         TMA producer of each CTA: its 128 rows of A and its 128 rows of B, six 32 KB stages.  All copies of both CTAs
 //                  count on the first CTA's barrier (their completion is what the issuer waits for)
 //   warp 1         of the first CTA: tcgen05.mma issuer; its commits free a stage, and hand over an accumulator, in both CTAs
-//   warps 4..11    epilogue of each CTA over its own two tiles, as in wholek_wide_kernel; both CTAs' warps free an
-//                  accumulator on the first CTA's barrier
+//   warps 4..19    epilogue of each CTA over its own two tiles, 32 rows x 64 columns of a unit each; both CTAs' warps free an
+//                  accumulator on the first CTA's barrier.  Sixteen warps instead of eight, because a warp's chain from tensor
+//                  memory to the store issues an instruction every eight to ten cycles: with K = 64, 16384 x 8192 outputs took
+//                  93 us with eight, 73 with sixteen, 56 with the epilogue as it stands (a library product: 48)
 // Two accumulators of 256 columns ping-pong.  Every wait is bounded, as in the other kernels; both CTAs meet before they leave.
 #pragma once
 #include "epi_linear.cuh"
@@ -25,16 +27,21 @@ namespace i8m {
 
 constexpr int LPR_STAGES = 6;
 constexpr int LPR_STAGE_BYTES = 2 * TILE_BYTES;
-constexpr int LPR_THREADS = 384;
-constexpr size_t LPR_SMEM = size_t(LPR_STAGES) * LPR_STAGE_BYTES + sizeof(Ctrl) + 8 * WARP_PATCH_BYTES + 1024;
+constexpr int LPR_EPI_WARPS = 16;
+constexpr int LPR_THREADS = 32 * (4 + LPR_EPI_WARPS);
+// 640 threads are launched with 96 registers each (65536 / 640, in eights): 61440, of which these take 60416
+constexpr int LPR_CTRL_REGS = 56, LPR_EPI_REGS = 104;
+static_assert(32 * (4 * LPR_CTRL_REGS + LPR_EPI_WARPS * LPR_EPI_REGS) <= LPR_THREADS * (65536 / LPR_THREADS / 8 * 8), "registers");
+constexpr size_t LPR_SMEM = size_t(LPR_STAGES) * LPR_STAGE_BYTES + sizeof(Ctrl) + LPR_EPI_WARPS * WARP_PATCH_BYTES + 1024;
+static_assert(LPR_SMEM <= 227 * 1024, "shared memory of a CTA");
 
 // Unit `linear` of the pairs of row tiles x pairs of column tiles, in the grouped order of decode_unit.
 __host__ __device__ __forceinline__ void decode_pair(const GemmGeom& g, int linear, int& row_pair, int& col_pair) {
-  const int row_pairs = (g.tiles_m + 1) / 2, cols = (g.tiles_n + 1) / 2, group = g.group / 2;
-  const int per_group = group * cols, grp = linear / per_group, in_group = linear - grp * per_group;
-  const int rows = row_pairs - grp * group < group ? row_pairs - grp * group : group;
-  col_pair = in_group / rows;
-  row_pair = grp * group + (in_group - col_pair * rows);
+  const unsigned row_pairs = unsigned(g.tiles_m + 1) / 2, cols = unsigned(g.tiles_n + 1) / 2, group = unsigned(g.group) / 2;
+  const unsigned per_group = group * cols, grp = unsigned(linear) / per_group, in_group = unsigned(linear) - grp * per_group;
+  const unsigned rows = row_pairs - grp * group < group ? row_pairs - grp * group : group;
+  col_pair = int(in_group / rows);
+  row_pair = int(grp * group + in_group % rows);
 }
 
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
@@ -74,14 +81,16 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
                "h"(uint16_t(3)) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive(uint32_t mapped_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped_bar) : "memory");
+// Arrive on a barrier of either CTA.  What it hands over is tensor memory that has been read (ordered by tcgen05's own fence), so
+// the release is left at CTA scope: at cluster scope the warp would wait here until its stores to global memory have arrived.
+__device__ __forceinline__ void pair_arrive(uint32_t mapped_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped_bar) : "memory");
 }
 
 template <typename E, int A_MN, int B_MN>
 __global__ void __launch_bounds__(LPR_THREADS, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, GemmGeom g,
-                   LinearArgs args) {
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, GemmGeom g, LinearArgs args) {
   using Epi = EpiLinear<E>;
   using Tiles = OperandTiles<E, A_MN, B_MN>;
   constexpr int STAGES = LPR_STAGES, STAGE_BYTES = LPR_STAGE_BYTES, ACC_COLS = 2 * TILE;
@@ -89,8 +98,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Ctrl* ctrl = reinterpret_cast<Ctrl*>(smem + STAGES * STAGE_BYTES);
-  uint8_t* patches = reinterpret_cast<uint8_t*>(ctrl + 1);
+  uint8_t* patches = smem + STAGES * STAGE_BYTES;            // on 512 bytes: the swizzle of what leaves
+  Ctrl* ctrl = reinterpret_cast<Ctrl*>(patches + LPR_EPI_WARPS * WARP_PATCH_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = int(blockIdx.x) & 1;
 
   if (threadIdx.x == 0) {
@@ -100,7 +109,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctrl->acc_empty[i]), 16);   // eight epilogue warps of each CTA
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 2 * LPR_EPI_WARPS);   // both CTAs' epilogue warps
     }
     ctrl->abort = 0;
     fence_mbar_init();
@@ -124,7 +133,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const int my_units = (units - pair_of + pairs - 1) / pairs, nkb = g.num_kb;
 
   if (warp < 4) {
-    setmaxnreg_dec<WKP_CTRL_REGS>();
+    setmaxnreg_dec<LPR_CTRL_REGS>();
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ producer
       const uint32_t full_at = cluster_map(full0, 0);        // the first CTA's barriers
@@ -190,12 +199,14 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
   } else {
     // -------------------------------------------------------------- epilogue
-    setmaxnreg_inc<WKP_EPI_REGS>();
+    setmaxnreg_inc<LPR_EPI_REGS>();
     const uint32_t freed = cluster_map(acce0, 0);            // the first CTA's barriers
     TileCtx t;
     t.b = 0;
     t.q = warp & 3; t.lane = lane;
-    t.ew = warp - 4; t.half = (warp - 4) >> 2;
+    t.ew = warp - 4;
+    const int slice = t.ew >> 2;                             // of the unit's 256 columns: 64
+    t.half = slice & 1;
     t.r = t.q * 32 + lane;
     t.ctrl = ctrl;
     t.red = ctrl->red; t.diag = ctrl->diag;
@@ -203,27 +214,31 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     t.wsm = patches + t.ew * WARP_PATCH_BYTES;
     t.c_begin = t.half * 2; t.c_end = t.half * 2 + 2;
     bool ok = true;
+    int rp = 0, cp = 0, next_rp = 0, next_cp = 0;
+    auto decode_next = [&](int j) {
+      decode_pair(g, pair_of + j * pairs, next_rp, next_cp);
+      Epi::expect_residual(g, args, (2 * next_rp + rank) * TILE + t.r, 2 * next_cp * TILE + 64 * slice);
+    };
+    if (my_units > 0) decode_next(0);
     for (int j = 0; j < my_units; ++j) {
-      int rp, cp;
-      decode_pair(g, pair_of + j * pairs, rp, cp);
+      rp = next_rp; cp = next_cp;
+      if (j + 1 < my_units) decode_next(j + 1);
       t.tm = 2 * rp + rank;
       t.row0 = t.tm * TILE;
       t.row = t.row0 + t.r;
       const int buf = j & 1;
-      if (ok) ok = mbar_wait_warp(accf0 + 8u * uint32_t(buf), uint32_t(j >> 1) & 1u, abort_flag);
+      ok = mbar_wait_warp(accf0 + 8u * uint32_t(buf), uint32_t(j >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-#pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        t.tn = 2 * cp + sub;
-        t.col0 = t.tn * TILE;
-        AccWholeK<KIND_F16, E, false> acc{g, t, tmem_base + (uint32_t(t.q * 32) << 16) + uint32_t(buf * ACC_COLS + sub * TILE)};
-        Epi::run(g, args, t, acc);
-      }
+      t.tn = 2 * cp + (slice >> 1);
+      t.col0 = t.tn * TILE;
+      AccWholeK<KIND_F16, E, false> acc{g, t, tmem_base + (uint32_t(t.q * 32) << 16) + uint32_t(buf * ACC_COLS + (slice >> 1) * TILE)};
+      Epi::run(g, args, &map_y, &map_z, t, acc);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) cluster_arrive(freed + 8u * uint32_t(buf));
+      if (lane == 0) pair_arrive(freed + 8u * uint32_t(buf));
     }
+    Epi::patch_free(WarpPatch{smem_u32(t.wsm), lane});       // copies from it end before the CTA does
     if (!ok && lane == 0) atomicCAS(g.status, 0u, unsigned(ST_EPILOGUE_TIMEOUT) | unsigned(blockIdx.x & 0xff));
   }
   __syncwarp();

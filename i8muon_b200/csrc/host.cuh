@@ -85,6 +85,8 @@ inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 // Rows may lie `pitch` elements apart (0: contiguous), and a K-major box may have fewer than 128 rows.
 int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn = 0, int pitch = 0,
                      int box_rows = 128);
+// Map over rows of 16-bit elements that are stored in blocks of 32 x 32, swizzled over 64 bytes.
+int make_block_map(CUtensorMap* map, void* ptr, int width, int rows, int pitch);
 int sm_count();   // of the current device, capped by i8m_set_cta_limit
 
 inline bool float_dtype_ok(int d) { return d == I8M_F32 || d == I8M_F16 || d == I8M_BF16; }

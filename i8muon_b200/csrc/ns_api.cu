@@ -60,6 +60,23 @@ int load_encode() {
   });
   return g_encode ? 0 : fail(I8M_E_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
 }
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, void* ptr, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+               const cuuint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
+  auto encode = [&] {
+    return g_encode(map, type, 3, ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {   // the first CUDA work of this thread: no runtime call has made a context current yet
+    int device;
+    CUDA_TRY(cudaGetDevice(&device));
+    CUDA_TRY(cudaSetDevice(device));
+    r = encode();
+  }
+  if (r != CUDA_SUCCESS) return fail(I8M_E_CUDA, "cuTensorMapEncodeTiled failed with code %d", int(r));
+  return 0;
+}
 }  // namespace
 
 int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int extent, int batch, int mn, int pitch, int box_rows) {
@@ -76,21 +93,14 @@ int make_operand_map(CUtensorMap* map, const void* ptr, int esize, int k, int ex
   cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(batch)};
   cuuint64_t strides[2] = {cuuint64_t(pitch) * esize, cuuint64_t(pitch) * esize * rows};
   cuuint32_t box[3] = {cuuint32_t(128 / esize), cuuint32_t(mn ? 128 / esize : box_rows), 1u};
-  cuuint32_t estr[3] = {1u, 1u, 1u};
-  auto encode = [&] {
-    return g_encode(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = encode();
-  if (r == CUDA_ERROR_INVALID_CONTEXT) {   // the first CUDA work of this thread: no runtime call has made a context current yet
-    int device;
-    CUDA_TRY(cudaGetDevice(&device));
-    CUDA_TRY(cudaSetDevice(device));
-    r = encode();
-  }
-  if (r != CUDA_SUCCESS) return fail(I8M_E_CUDA, "cuTensorMapEncodeTiled failed with code %d", int(r));
-  return 0;
+  return encode_map(map, dt, const_cast<void*>(ptr), dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int make_block_map(CUtensorMap* map, void* ptr, int width, int rows, int pitch) {
+  if (int rc = load_encode()) return rc;
+  const cuuint64_t dims[3] = {cuuint64_t(width), cuuint64_t(rows), 1u};
+  const cuuint64_t strides[2] = {cuuint64_t(pitch) * 2, cuuint64_t(pitch) * 2 * rows};
+  const cuuint32_t box[3] = {32u, 32u, 1u};
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace i8m

@@ -298,6 +298,29 @@ def test_linear_over_many_tiles_and_long_sums(cuda_device, shape):
     check_linear(*linear_inputs(*shape, torch.bfloat16, cuda_device), "gelu")
 
 
+@pytest.mark.parametrize("shape", [(5003, 72, 2056), (5003, 80, 2057), (2600, 40, 4328)])
+@pytest.mark.parametrize("checkpoint", (None, "int8"))
+def test_linear_units_at_the_edges(cuda_device, shape, checkpoint):
+    """Products in units of 256 x 256 whose last units reach beyond the rows and the columns."""
+    from i8muon_b200 import native
+    from i8muon_b200.engine import status_word
+    rows, inner, outer = shape
+    x, w, b, r, dy = linear_inputs(*shape, torch.float16, cuda_device)
+    check_linear(x, w, b, r, dy, "silu", checkpoint)
+    # nothing behind the last row of y and of the kept pre-activation is written, and nothing in front
+    pitch = -(-outer // 8) * 8
+    y = torch.full((rows * outer + 1024,), 77, dtype=torch.float16, device=cuda_device)
+    z = torch.full((rows * pitch + 1024,), 77, dtype=torch.float16, device=cuda_device)
+    size = native.linear_workspace_bytes(x.data_ptr(), w.data_ptr(), rows, inner, outer)
+    work = torch.empty(size, dtype=torch.uint8, device=cuda_device)
+    native.call("i8m_linear", x.data_ptr(), w.data_ptr(), b.data_ptr(), r.data_ptr(), y[512:].data_ptr(), z[512:].data_ptr(), None, None, -1, 5, rows,
+                inner, outer, native.F16, work.data_ptr(), size, status_word(cuda_device).data_ptr(), torch.cuda.current_stream().cuda_stream)
+    check_status()
+    for t, count in ((y, rows * outer), (z, rows * pitch)):
+        assert (t[:512] == 77).all() and (t[512 + count:] == 77).all()
+    assert torch.equal(y[512:512 + rows * outer].view(rows, outer), linear(x, w, b, activation="silu", residual=r))
+
+
 def test_linear_takes_any_strides_and_leading_dimensions(cuda_device):
     dtype = torch.bfloat16
     base, wbase = normal((4, 6, 80), 1, dtype, cuda_device), normal((50, 160), 2, dtype, cuda_device, 0.1)
