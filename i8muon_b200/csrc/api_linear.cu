@@ -5,6 +5,7 @@
 #include "gemm_linear_split.cuh"
 #include "layers.cuh"
 
+#include <algorithm>
 #include <cmath>
 
 using namespace i8m;
@@ -17,13 +18,16 @@ struct Operand {
   int pitch, mn;
 };
 
-// How a product is carried out: on pairs of SMs in units of 256 x 256 (bn 0), or by the split kernel with tiles of 128 features x
-// bn rows.
+// How a product is carried out: on pairs of SMs in units of 256 x 256 (bn 0), K cut into `split` parts, or by the split kernel with
+// tiles of 128 features x bn rows and K cut over `split` CTAs.
 struct Plan {
   int bn, split;
 };
+// Parts are FP32 results in the workspace, at most this much.
+constexpr size_t MOST_PART_BYTES = size_t(64) << 20;
+inline size_t part_bytes(int m, int n) { return size_t(m) * pad_to(n, 8) * 4; }
 // The least of an estimate in nanoseconds.  Pairs: 6 us, and 0.365 us per K block of a wave of units, at least 1.85 us (an epilogue)
-// for every wave but the first.  Split kernel: 4.5 us and 25 ns
+// for every wave but the first; in parts, 3 us more for the launch that folds them and 8 TB/s for what it moves.  Split kernel: 4.5 us and 25 ns
 // per column of the tile for its start, sums and end, 4 us for every further wave, and per K block 14 ns for each KB that the
 // CTA takes in, at least 0.27 us, or 17 ns per KB where two CTAs share an SM.  Both: beside the time that DRAM takes for the
 // operands (as the root of the sum of squares: neither hides the other fully).
@@ -31,13 +35,18 @@ struct Plan {
 // 16 x 4096 -> 14336 29 / 23.6 (16, 2); 256 x 4096 -> 4096 26.6 / 17.2 (128, 4); 512 27.2 / 23.1 (128, 2); 1024 28.7 / 37.6 (128, 1);
 // 333 x 1008 -> 520 11.4 / 6.5 (64, 4); 1024 x 768 -> 768 10.2 / 9.0 (32, 1); 2048 x 1024 -> 1024 12.3 / 12.9 (64, 1);
 // 300 x 8192 -> 256 44.6 / 10.8 (64, 8).
-Plan plan_product(int rows, int features, int k, bool rows_mn, int sms) {
+Plan plan_product(int rows, int features, int k, bool rows_mn, int sms, size_t room) {
   const int num_kb = cdiv(2LL * k, 128);
   const double dram = 2.0 * k * ((double)rows + features) / 6200.0;
   auto beside_dram = [&](double v) { return std::sqrt(v * v + dram * dram); };
   const long long units = (long long)cdiv(rows, 2 * TILE) * cdiv(features, 2 * TILE), pairs = std::max(1, sms / 2);
   Plan best{0, 1};
-  double cost = 6000 + beside_dram(num_kb * 365.0 + ((units + pairs - 1) / pairs - 1) * std::max(1850.0, num_kb * 365.0));
+  double cost = 1e30;
+  for (int parts = 1; parts <= 64 && (parts == 1 || (4 * parts <= num_kb && parts * part_bytes(rows, features) <= room)); ++parts) {
+    const double block = (num_kb + parts - 1) / parts * 365.0, fold = 3000 + 2.0 * parts * part_bytes(rows, features) / 8000.0;
+    const double c = 6000 + beside_dram(block + ((units * parts + pairs - 1) / pairs - 1) * std::max(1850.0, block)) + (parts > 1 ? fold : 0);
+    if (c < cost) { cost = c; best = {0, parts}; }
+  }
   for (int bn = rows_mn ? 64 : 16; bn <= 128; bn *= 2) {
     const long long split_tiles = (long long)cdiv(features, TILE) * cdiv(rows, bn), kilobytes = 16 + bn / 8;
     for (int split = 1; split <= 8 && split <= num_kb; split *= 2) {
@@ -94,16 +103,16 @@ int product_split(const Plan& plan, const Operand& a, const Operand& b, int m, i
 // Rows of `width` 16-bit elements, one behind the other, that tensor copies can address.
 bool addressable(const void* p, int width) { return width % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename E, int A_MN, int B_MN>
+template <typename E, int A_MN, int B_MN, bool PARTS = false>
 int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g, LinearArgs args, unsigned pairs,
                 cudaStream_t stream, const char* name) {
   CUtensorMap my = ma, mz = ma;          // what is not stored through its map has none
-  args.y_blocks = addressable(args.y, g.n);
+  args.y_blocks = !PARTS && addressable(args.y, g.n);
   if (args.y_blocks)
     if (int rc = make_block_map(&my, args.y, g.n, g.m, g.n)) return rc;
   if (args.z != nullptr)
     if (int rc = make_block_map(&mz, args.z, args.z_pitch, g.m, args.z_pitch)) return rc;
-  auto kernel = linear_pair_kernel<E, A_MN, B_MN>;
+  auto kernel = linear_pair_kernel<E, A_MN, B_MN, PARTS>;
   static SmemAllowed allowed;
   if (int rc = allow_smem(allowed, kernel, LPR_SMEM)) return rc;
   launch_clusters(kernel, 2, 2 * pairs, LPR_THREADS, LPR_SMEM, stream, ma, mb, my, mz, g, args);
@@ -111,10 +120,10 @@ int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g,
   return 0;
 }
 
-// out (m, n) = a b^T over k.
+// out (m, n) = a b^T over k.  `parts`: room for FP32 parts of it, of `room` bytes (none: the sum stays whole).
 template <typename E>
-int product(const Operand& a, const Operand& b, int m, int n, int k, const LinearArgs& args, unsigned* status, cudaStream_t stream,
-            const char* name) {
+int product(const Operand& a, const Operand& b, int m, int n, int k, LinearArgs args, float* parts, size_t room, unsigned* status,
+            cudaStream_t stream, const char* name) {
   GemmGeom g{};
   g.batch = 1; g.m = g.lm = m; g.n = g.ln = n; g.k = k;
   g.tiles_m = cdiv(m, TILE); g.tiles_n = cdiv(n, TILE);
@@ -126,16 +135,26 @@ int product(const Operand& a, const Operand& b, int m, int n, int k, const Linea
   g.a_mn = a.mn; g.b_mn = b.mn;
   g.group = wide_group(2LL * k);
   g.a_raw = a.p; g.b_raw = b.p; g.status = status;
-  const Plan plan = plan_product(m, n, k, a.mn, sm_count());
+  const Plan plan = plan_product(m, n, k, a.mn, sm_count(), room);
   if (plan.bn) return product_split<E>(plan, a, b, m, n, k, args, status, stream, name);
   CUtensorMap ma, mb;
   if (int rc = make_operand_map(&ma, a.p, 2, k, m, 1, a.mn, a.pitch)) return rc;
   if (int rc = make_operand_map(&mb, b.p, 2, k, n, 1, b.mn, b.pitch)) return rc;
   const long long units = (long long)cdiv(g.tiles_m, 2) * cdiv(g.tiles_n, 2);
-  const unsigned pairs_of_sms = unsigned(std::min<long long>(units, std::max(1, sm_count() / 2)));
-  if (!a.mn && !b.mn) return launch_pair<E, 0, 0>(ma, mb, g, args, pairs_of_sms, stream, name);
-  if (!a.mn) return launch_pair<E, 0, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
-  return launch_pair<E, 1, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
+  const unsigned pairs_of_sms = unsigned(std::min<long long>(units * plan.split, std::max(1, sm_count() / 2)));
+  if (plan.split == 1) {
+    if (!a.mn && !b.mn) return launch_pair<E, 0, 0>(ma, mb, g, args, pairs_of_sms, stream, name);
+    if (!a.mn) return launch_pair<E, 0, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
+    return launch_pair<E, 1, 1>(ma, mb, g, args, pairs_of_sms, stream, name);
+  }
+  args.parts = parts; args.part_count = plan.split; args.z_pitch = pad_to(n, 8);
+  if (int rc = a.mn ? launch_pair<E, 1, 1, true>(ma, mb, g, args, pairs_of_sms, stream, name)      // room is given to gradients alone
+                    : launch_pair<E, 0, 1, true>(ma, mb, g, args, pairs_of_sms, stream, name)) return rc;
+  const long long octets = (long long)m * (args.z_pitch / 8);
+  launch(parts_fold_kernel<E>, unsigned(std::min<long long>((octets + 255) / 256, 148LL * 8)), 256, 0, stream, parts, static_cast<E*>(args.y),
+         plan.split, m, n, args.z_pitch, addressable(args.y, n));
+  LAUNCH_CHECK("parts_fold");
+  return 0;
 }
 template <typename... A>
 int product_of(int dtype, A&&... args) {
@@ -178,8 +197,8 @@ struct ForwardPieces {
 };
 struct BackwardPieces {
   void *w = nullptr, *x = nullptr, *dz = nullptr;
-  float* partials = nullptr;
-  size_t bytes;
+  float *partials = nullptr, *parts = nullptr;
+  size_t bytes, room = 0;
   BackwardPieces(void* base, const void* dy, const void* x_in, const void* w_in, int rows, int inner, int outer, int activation,
                  int format, bool dx, bool dw, bool db) {
     Carver c{static_cast<uint8_t*>(base)};
@@ -188,6 +207,14 @@ struct BackwardPieces {
     if (dw && (format >= 0 || !addressable(x_in, inner))) x = c.take(rows_bytes(rows, pitch));
     if ((dx || dw) && (activation != ACT_NONE || !addressable(dy, outer))) dz = c.take(rows_bytes(rows, pad_to(outer, 8)));
     if (db) partials = static_cast<float*>(c.take(size_t(dz_bands(rows, outer)) * 2 * outer * sizeof(float)));
+    // a product may be cut for 148 SMs; where fewer are in use it is cut to fit
+    auto parts_of = [&](int m, int n, int k, bool mn) {
+      const Plan plan = plan_product(m, n, k, mn, 148, MOST_PART_BYTES);
+      return plan.bn == 0 && plan.split > 1 ? plan.split * part_bytes(m, n) : size_t(0);
+    };
+    if (dx) room = parts_of(rows, inner, outer, false);
+    if (dw) room = std::max(room, parts_of(outer, inner, rows, true));
+    if (room) parts = static_cast<float*>(c.take(room));
     bytes = c.used;
   }
 };
@@ -211,6 +238,7 @@ extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, c
   const ForwardPieces pieces(workspace, x, weight, rows, inner, outer);
   if (pieces.bytes && (!workspace || workspace_bytes < pieces.bytes))
     return fail(I8M_E_WORKSPACE, "linear: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, pieces.bytes);
+  if (pieces.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return fail(I8M_E_ARGUMENT, "linear: workspace is not 16-byte aligned");
   const int pitch = pad_to(inner, 8);
   if (int rc = pitch_rows(x, pieces.x, rows, weight, pieces.w, outer, dtype, inner, pitch, S(stream))) return rc;
   LinearArgs a{};
@@ -219,7 +247,7 @@ extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, c
   a.codes = format >= 0 ? static_cast<uint8_t*>(z_codes) : nullptr; a.exponents = static_cast<uint8_t*>(z_exponents);
   a.groups = eight_groups(outer); a.format = format; a.activation = activation;
   return product_of(dtype, Operand{pieces.x ? pieces.x : x, pitch, 0}, Operand{pieces.w ? pieces.w : weight, pitch, 0}, rows, outer,
-                    inner, a, status, S(stream), "linear");
+                    inner, a, nullptr, size_t(0), status, S(stream), "linear");
 }
 
 extern "C" int i8m_linear_backward_workspace_bytes(const void* dy, const void* x, const void* weight, int rows, int inner, int outer,
@@ -247,6 +275,7 @@ extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_
   const BackwardPieces pieces(workspace, dy, x, weight, rows, inner, outer, activation, format, dx, dweight, dbias);
   if (pieces.bytes && (!workspace || workspace_bytes < pieces.bytes))
     return fail(I8M_E_WORKSPACE, "linear_backward: workspace %zu < %zu bytes", workspace ? workspace_bytes : 0, pieces.bytes);
+  if (pieces.bytes && (reinterpret_cast<uintptr_t>(workspace) & 31u)) return fail(I8M_E_ARGUMENT, "linear_backward: workspace is not 32-byte aligned");
   const int inner_pitch = pad_to(inner, 8), outer_pitch = pad_to(outer, 8);
 
   if (pieces.dz || dbias) {
@@ -264,14 +293,14 @@ extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_
   if (dx) {
     a.y = dx;
     if (int rc = product_of(dtype, Operand{dz, outer_pitch, 0}, Operand{pieces.w ? pieces.w : weight, inner_pitch, 1}, rows, inner,
-                            outer, a, status, S(stream), "linear_dx")) return rc;
+                            outer, a, pieces.parts, pieces.room, status, S(stream), "linear_dx")) return rc;
   }
   if (dweight) {
     if (restored)
       if (int rc = eight_restore(x_codes, x_exponents, rows, inner, format, pieces.x, dtype, inner_pitch, S(stream))) return rc;
     a.y = dweight;
     if (int rc = product_of(dtype, Operand{dz, outer_pitch, 1}, Operand{pieces.x ? pieces.x : x, inner_pitch, 1}, outer, inner, rows,
-                            a, status, S(stream), "linear_dweight")) return rc;
+                            a, pieces.parts, pieces.room, status, S(stream), "linear_dweight")) return rc;
   }
   return 0;
 }

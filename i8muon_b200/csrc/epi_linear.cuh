@@ -23,6 +23,8 @@ struct LinearArgs {
   uint8_t* exponents;
   int z_pitch, groups, format, activation;
   int y_blocks;            // rows of y start on 16 bytes: blocks leave as tensor copies
+  float* parts;            // a sum cut into `part_count` runs of K blocks: (part_count, lm, z_pitch) FP32 instead of y, or NULL
+  int part_count;
 };
 
 __device__ __forceinline__ bool on_16_bytes(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -102,6 +104,28 @@ struct EpiLinear {
     const E* r = static_cast<const E*>(a.residual) + size_t(row) * g.ln;
     asm volatile("prefetch.global.L2 [%0];" ::"l"(r + col));
     asm volatile("prefetch.global.L2 [%0];" ::"l"(r + min(col + 63, g.ln - 1)));
+  }
+
+  // This warp's blocks as FP32 rows of one part of the sum.
+  template <class Acc>
+  static __device__ __forceinline__ void park(const GemmGeom& g, const Args& a, int part, const TileCtx& t, const Acc& acc) {
+#pragma unroll 1
+    for (int c = t.c_begin; c < t.c_end; ++c) {
+      const int colb = t.col0 + c * 32;
+      if (colb >= g.ln) continue;                                  // uniform over the warp
+      uint32_t v[32];
+      acc.load(c, v);
+      float* line = a.parts + (size_t(part) * g.lm + t.row) * a.z_pitch + colb;
+      if (t.row >= g.lm) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (colb + 8 * q >= a.z_pitch) continue;
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[8 * q + j]);
+        store8<float>(line + 8 * q, f);
+      }
+    }
   }
 
   // This warp's blocks of the tile.

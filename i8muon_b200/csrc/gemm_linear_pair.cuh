@@ -44,6 +44,22 @@ __host__ __device__ __forceinline__ void decode_pair(const GemmGeom& g, int line
   row_pair = int(grp * group + in_group % rows);
 }
 
+// Item `linear` of the units x parts of the sum: its unit and its run of K blocks.  Without PARTS a sum is whole.
+struct PairItem { int row_pair, col_pair, part, kb0, kb1; };
+template <bool PARTS>
+__host__ __device__ __forceinline__ PairItem decode_item(const GemmGeom& g, int part_count, int linear) {
+  PairItem it{0, 0, 0, 0, g.num_kb};
+  if (PARTS) {
+    const int unit = linear / part_count;
+    it.part = linear - unit * part_count;
+    it.kb0 = int((long long)g.num_kb * it.part / part_count);
+    it.kb1 = int((long long)g.num_kb * (it.part + 1) / part_count);
+    linear = unit;
+  }
+  decode_pair(g, linear, it.row_pair, it.col_pair);
+  return it;
+}
+
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
 }
@@ -87,7 +103,37 @@ __device__ __forceinline__ void pair_arrive(uint32_t mapped_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped_bar) : "memory");
 }
 
-template <typename E, int A_MN, int B_MN>
+// A product whose units are fewer than the pairs, or fill their last wave badly, is cut along K: a pair takes one part of a unit's K
+// blocks and parks FP32 sums, which parts_fold_kernel adds up in the order of the parts.
+template <typename E>
+__global__ void __launch_bounds__(256)
+parts_fold_kernel(const float* __restrict__ parts, E* __restrict__ out, int part_count, int rows, int width, int pitch, bool vectors) {
+  pdl_wait();
+  const int octets = pitch / 8;
+  const long long total = (long long)rows * octets, apart = (long long)rows * pitch;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / octets;
+    const int col = int(i - row * octets) * 8;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < part_count; ++p) {
+      const float4* f = reinterpret_cast<const float4*>(parts + p * apart + row * pitch + col);
+      const float4 a = f[0], b = f[1];
+      s[0] += a.x; s[1] += a.y; s[2] += a.z; s[3] += a.w;
+      s[4] += b.x; s[5] += b.y; s[6] += b.z; s[7] += b.w;
+    }
+    E* to = out + row * width + col;
+    if (vectors) {
+      store8<E>(to, s);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < width) to[j] = round_to<E>(s[j]);
+    }
+  }
+}
+
+template <typename E, int A_MN, int B_MN, bool PARTS>
 __global__ void __launch_bounds__(LPR_THREADS, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_z, GemmGeom g, LinearArgs args) {
@@ -129,8 +175,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   const uint32_t full0 = smem_u32(&ctrl->full[0]), empty0 = smem_u32(&ctrl->empty[0]);
   const uint32_t accf0 = smem_u32(&ctrl->acc_full[0]), acce0 = smem_u32(&ctrl->acc_empty[0]);
 
-  const int units = (g.tiles_m + 1) / 2 * ((g.tiles_n + 1) / 2), pairs = int(gridDim.x) / 2, pair_of = int(blockIdx.x) / 2;
-  const int my_units = (units - pair_of + pairs - 1) / pairs, nkb = g.num_kb;
+  const int units = (g.tiles_m + 1) / 2 * ((g.tiles_n + 1) / 2) * (PARTS ? args.part_count : 1), pairs = int(gridDim.x) / 2, pair_of = int(blockIdx.x) / 2;
+  const int my_units = (units - pair_of + pairs - 1) / pairs;
 
   if (warp < 4) {
     setmaxnreg_dec<LPR_CTRL_REGS>();
@@ -142,10 +188,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       bool ok = true;
       const int todo = (g.debug_simt & 0x100) ? 0 : my_units;  // test hook: issue nothing
       for (int j = 0; j < todo && ok; ++j) {
-        int rp, cp;
-        decode_pair(g, pair_of + j * pairs, rp, cp);
-        const int r0 = (2 * rp + rank) * TILE, n0 = (2 * cp + rank) * TILE;
-        for (int kb = 0; kb < nkb; ++kb) {
+        const PairItem it = decode_item<PARTS>(g, args.part_count, pair_of + j * pairs);
+        const int r0 = (2 * it.row_pair + rank) * TILE, n0 = (2 * it.col_pair + rank) * TILE;
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
           if (wrap > 0) {
             ok = mbar_wait(empty0 + 8u * uint32_t(ring), (wrap - 1) & 1u, abort_flag);
             if (!ok) break;
@@ -181,7 +226,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           tc_fence_after();
         }
         const uint32_t d = tmem_base + uint32_t(buf * ACC_COLS);
-        for (int kb = 0; kb < nkb; ++kb) {
+        const PairItem it = decode_item<PARTS>(g, args.part_count, pair_of + j * pairs);
+        for (int kb = it.kb0; kb < it.kb1; ++kb) {
           ok = mbar_wait(full0 + 8u * uint32_t(ring), wrap & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
@@ -189,7 +235,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           const uint64_t adesc = Tiles::desc_a(sa), bdesc = Tiles::desc_b(sa + TILE_BYTES);
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            pair_umma(d, adesc + uint64_t(ks) * Tiles::A_STEP, bdesc + uint64_t(ks) * Tiles::B_STEP, IDESC, kb > 0 || ks > 0);
+            pair_umma(d, adesc + uint64_t(ks) * Tiles::A_STEP, bdesc + uint64_t(ks) * Tiles::B_STEP, IDESC, kb > it.kb0 || ks > 0);
           pair_commit(empty0 + 8u * uint32_t(ring));
           if (++ring == STAGES) { ring = 0; ++wrap; }
         }
@@ -214,26 +260,27 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     t.wsm = patches + t.ew * WARP_PATCH_BYTES;
     t.c_begin = t.half * 2; t.c_end = t.half * 2 + 2;
     bool ok = true;
-    int rp = 0, cp = 0, next_rp = 0, next_cp = 0;
+    PairItem next{};
     auto decode_next = [&](int j) {
-      decode_pair(g, pair_of + j * pairs, next_rp, next_cp);
-      Epi::expect_residual(g, args, (2 * next_rp + rank) * TILE + t.r, 2 * next_cp * TILE + 64 * slice);
+      next = decode_item<PARTS>(g, args.part_count, pair_of + j * pairs);
+      Epi::expect_residual(g, args, (2 * next.row_pair + rank) * TILE + t.r, 2 * next.col_pair * TILE + 64 * slice);
     };
     if (my_units > 0) decode_next(0);
     for (int j = 0; j < my_units; ++j) {
-      rp = next_rp; cp = next_cp;
+      const PairItem it = next;
       if (j + 1 < my_units) decode_next(j + 1);
-      t.tm = 2 * rp + rank;
+      t.tm = 2 * it.row_pair + rank;
       t.row0 = t.tm * TILE;
       t.row = t.row0 + t.r;
       const int buf = j & 1;
       ok = mbar_wait_warp(accf0 + 8u * uint32_t(buf), uint32_t(j >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
-      t.tn = 2 * cp + (slice >> 1);
+      t.tn = 2 * it.col_pair + (slice >> 1);
       t.col0 = t.tn * TILE;
       AccWholeK<KIND_F16, E, false> acc{g, t, tmem_base + (uint32_t(t.q * 32) << 16) + uint32_t(buf * ACC_COLS + (slice >> 1) * TILE)};
-      Epi::run(g, args, &map_y, &map_z, t, acc);
+      if constexpr (PARTS) Epi::park(g, args, it.part, t, acc);
+      else Epi::run(g, args, &map_y, &map_z, t, acc);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) pair_arrive(freed + 8u * uint32_t(buf));

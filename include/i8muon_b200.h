@@ -320,7 +320,8 @@ int i8m_linear(const void* x_device, const void* weight_device, const void* bias
 /* Gradients of the above (the residual's is dy itself); dx, dweight, dbias may each be NULL.  dz = dy act'(z) at the kept z,
  * rounded to `dtype` as the operand of dx = dz weight and dweight = dz^T x; dbias sums the unrounded dz over bands of rows in
  * a fixed order.  x, or its codes (i8m_activation_quant) where `format` names a format, serves dweight; z or its codes serve an
- * activation.  dx, dweight and dbias in the arguments of the query are truth values. */
+ * activation.  dx, dweight and dbias in the arguments of the query are truth values.  workspace (32-byte aligned): dz, copies as
+ * above, bands of dbias, and up to 64 MB of FP32 parts where a gradient is a long sum into few tiles. */
 int i8m_linear_backward_workspace_bytes(const void* dy_device, const void* x_device, const void* weight_device, int rows, int inner,
                                         int outer, int activation, int format, int dx, int dweight, int dbias, size_t* bytes);
 int i8m_linear_backward(const void* dy_device, const void* x_device, const void* x_codes_device, const void* x_exponents_device,

@@ -321,6 +321,12 @@ def test_linear_units_at_the_edges(cuda_device, shape, checkpoint):
     assert torch.equal(y[512:512 + rows * outer].view(rows, outer), linear(x, w, b, activation="silu", residual=r))
 
 
+@pytest.mark.parametrize("shape, checkpoint", [((16384, 768, 768), None), ((20000, 520, 513), None), ((16384, 256, 300), "fp8"), ((300, 768, 16384), None)])
+def test_linear_sums_in_parts(cuda_device, shape, checkpoint):
+    """Gradients that are long sums into few units: cut along the sum."""
+    check_linear(*linear_inputs(*shape, torch.bfloat16, cuda_device, residual=False), None, checkpoint)
+
+
 def test_linear_takes_any_strides_and_leading_dimensions(cuda_device):
     dtype = torch.bfloat16
     base, wbase = normal((4, 6, 80), 1, dtype, cuda_device), normal((50, 160), 2, dtype, cuda_device, 0.1)
