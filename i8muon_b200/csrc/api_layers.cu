@@ -97,8 +97,11 @@ static int linear_dz_typed(const LinearDz& d, cudaStream_t stream) {
                               static_cast<const uint8_t*>(d.exponents), d.z_pitch, eight_groups(d.width)};
   float* partials = d.db ? d.partials : nullptr;
   const bool aligned = d.width % 8 == 0 && on_octets(d.dy, 2);
-  DISPATCH_FORMAT(d.format, F, {
-    auto kernel = aligned ? linear_dz_kernel<E, F, true> : linear_dz_kernel<E, F, false>;
+  const bool active = d.activation != ACT_NONE;
+  DISPATCH_FORMAT(active ? d.format : -1, F, {
+    auto kernel = aligned ? linear_dz_kernel<E, F, true, true> : linear_dz_kernel<E, F, false, true>;
+    if constexpr (F < 0)
+      if (!active) kernel = aligned ? linear_dz_kernel<E, F, true, false> : linear_dz_kernel<E, F, false, false>;
     launch(kernel, dim3(cdiv(d.width, 256), bands), 32 * DZ_WARPS, 0, stream, static_cast<const E*>(d.dy), kept,
            static_cast<E*>(d.dz), partials, d.rows, d.width, d.dz_pitch, band, d.activation);
   });

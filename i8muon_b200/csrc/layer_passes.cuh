@@ -239,32 +239,47 @@ struct PreActivation {
 };
 // dz = dy act'(z) (dz may be NULL) and, where partials is not NULL, its sums over bands of rows for the bias's gradient: partials
 // (bands, 2, width), of which the first line of a band is written.  A lane takes eight columns, a warp 256 of a row, the
-// block's warps rows one after the other, DZ_ROWS of them on their way at a time.  ALIGNED: rows of dy are whole octets on 16
-// bytes, as those of z and dz always are.  Bound by HBM (6 bytes per element, 5 with codes); the special functions of an
+// block's warps rows one after the other, DZ_ROWS of them on their way at a time (three and three blocks per SM where there is an
+// activation: 8192 x 14336 with GELU took 133 us with four rows and two blocks, 126 with two and four, 119 so).  ALIGNED: rows of dy are whole octets on 16
+// bytes, as those of z and dz always are; ACTIVE: there is an activation.  Bound by HBM (6 bytes per element, 5 with codes); the special functions of an
 // activation come second.
-constexpr int DZ_WARPS = 8, DZ_ROWS = 4;
-template <typename E, int FORMAT, bool ALIGNED>
-__global__ void __launch_bounds__(32 * DZ_WARPS)
+constexpr int DZ_WARPS = 8;
+template <typename E, int FORMAT, bool ALIGNED, bool ACTIVE>
+__global__ void __launch_bounds__(32 * DZ_WARPS, ACTIVE ? 3 : 4)
 linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict__ dz, float* __restrict__ partials, long long rows,
                  int width, int dz_pitch, long long band, int activation) {
+  constexpr int DZ_ROWS = ACTIVE ? 3 : 4;
   __shared__ float sums[DZ_WARPS][256];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * 8;
   const long long first = blockIdx.y * band, last = first + band < rows ? first + band : rows;
   unsigned long long sum[4] = {0ull, 0ull, 0ull, 0ull};
   if (col < width) {
-    with_activation(activation, [&](auto act) {
+    auto rows_of = [&](auto act) {
       constexpr int ACT = decltype(act)::value;
       for (long long row = first + warp; row < last; row += DZ_WARPS * DZ_ROWS) {
         Octet<E> d[DZ_ROWS];
         uint4 z[DZ_ROWS];
         [[maybe_unused]] uint32_t byte[DZ_ROWS];
+        [[maybe_unused]] uint32_t words[ALIGNED ? 1 : DZ_ROWS][Octet<E>::WORDS + 7];
+        // all rows exist and so do all pieces: one decision, and the rows' loads are on their way together
+        const long long end_row = row + (DZ_ROWS - 1) * DZ_WARPS;
+        [[maybe_unused]] const bool together = !ALIGNED && end_row < last &&
+                              load_inside_fits<E>(dy + row * width + col, dy + end_row * width + col, dy, dy + rows * width);
+        if constexpr (!ALIGNED) {
+          if (together) {
+#pragma unroll
+            for (int r = 0; r < DZ_ROWS; ++r) load_inside<E>(words[r], dy + (row + r * DZ_WARPS) * width + col);
+#pragma unroll
+            for (int r = 0; r < DZ_ROWS; ++r) shift_inside<E>(d[r], words[r], dy + (row + r * DZ_WARPS) * width + col, width - col);
+          }
+        }
 #pragma unroll
         for (int r = 0; r < DZ_ROWS; ++r) {
           const long long at = row + r * DZ_WARPS;
           if (at >= last) continue;
           if constexpr (ALIGNED) d[r].load(dy + at * width + col);
-          else load_any<E>(d[r], dy + at * width + col, width - col, dy, dy + rows * width);
+          else if (!together) load_any<E>(d[r], dy + at * width + col, width - col, dy, dy + rows * width);
           if constexpr (ACT == ACT_NONE) continue;
           if constexpr (FORMAT >= 0) {
             const uint2 c = *reinterpret_cast<const uint2*>(kept.codes + at * kept.groups * EIGHT_GROUP + col);
@@ -293,7 +308,9 @@ linear_dz_kernel(const E* __restrict__ dy, PreActivation<E> kept, E* __restrict_
           if (dz != nullptr) store8<E>(dz + at * dz_pitch + col, v);
         }
       }
-    });
+    };
+    if constexpr (ACTIVE) with_activation(activation, rows_of);
+    else rows_of(std::integral_constant<int, ACT_NONE>{});
   }
   if (partials == nullptr) return;
 #pragma unroll

@@ -115,6 +115,38 @@ __device__ __forceinline__ void load_any(Octet<E>& o, const E* p, int n, const E
   if (n < 8) o.cut(n);
 }
 
+// Eight elements at p without a branch, for loads that shall be on their way together: all pieces that load_inside_fits names exist.
+template <typename E>
+__device__ __forceinline__ bool load_inside_fits(const E* first, const E* last, const E* begin, const E* end) {
+  constexpr uintptr_t BYTES = 16 * (Octet<E>::WORDS / 4 + 1);
+  return (reinterpret_cast<uintptr_t>(first) & ~uintptr_t(15)) >= reinterpret_cast<uintptr_t>(begin) &&
+         (reinterpret_cast<uintptr_t>(last) & ~uintptr_t(15)) + BYTES <= reinterpret_cast<uintptr_t>(end);
+}
+template <typename E>
+__device__ __forceinline__ void load_inside(uint32_t (&w)[Octet<E>::WORDS + 7], const E* p) {
+  const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+#pragma unroll
+  for (int k = 0; k < Octet<E>::WORDS / 4 + 1; ++k) {
+    const uint4 v = base[k];
+    w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
+  }
+  w[Octet<E>::WORDS + 4] = w[Octet<E>::WORDS + 5] = w[Octet<E>::WORDS + 6] = 0u;
+}
+template <typename E>
+__device__ __forceinline__ void shift_inside(Octet<E>& o, uint32_t (&w)[Octet<E>::WORDS + 7], const E* p, int n) {
+  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p) & 15u);
+  if constexpr (Octet<E>::WORDS == 8) {
+    shift_words<8>(w, off >> 2);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o.q[k] = w[k];
+  } else {
+    shift_words<5>(w, off >> 2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o.q[k] = __funnelshift_r(w[k], w[k + 1], (off & 2u) * 8u);
+  }
+  if (n < 8) o.cut(n);
+}
+
 // Stores the n (0 .. 8) first elements of every lane's octet.  All lanes call it; lane l's octet starts 8 l elements behind lane
 // 0's, and only the last lane that has elements may have fewer than eight.
 template <typename E>
