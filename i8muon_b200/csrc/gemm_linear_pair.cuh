@@ -4,10 +4,10 @@
 // CTA, multiplies 256 rows of A - 128 in each CTA's shared memory - with 256 rows of B, of which each CTA holds half, and
 // leaves 128 x 256 outputs in each CTA's tensor memory.  Against wholek_wide_kernel, whose CTA needs 48 KB of operands for the
 // same 128 x 256 outputs of a K block, a CTA takes in 32 KB: two thirds of the traffic from L2 and of the writes to shared
-// memory, which at the power limit is clock rate as well.  8192 x 2048 -> 8192 BF16: 206 -> 188 us in a burst, 225 -> 213 us
+// memory, which at the power limit is clock rate as well.  8192 x 2048 -> 8192 BF16: 206 -> 185 us in a burst, 225 -> 215 us
 // over half a second (a library product: 176 and 205); with an INT8 copy of the pre-activation 247 -> 203 in a burst.
-// What bounds it: the tensor pipe, 84.6 % of the active cycles (a K block takes 597 cycles for 512 of tensor work; a library product
-// of these sizes 85.5 %).  An epilogue with GELU costs 14 % (74.3 %), an INT8 copy of the pre-activation 6 % (80.2 %): they run
+// What bounds it: the tensor pipe, 85 % of the active cycles (a K block takes 595 cycles for 512 of tensor work; a library product
+// of these sizes 85.5 %).  An epilogue with GELU costs 14 % (74 %), an INT8 copy of the pre-activation 8 % (79 %): they run
 // beside the K loop of the next unit, the last one of a CTA alone.
 //
 //   warp 0         TMA producer of each CTA: its 128 rows of A and its 128 rows of B, six 32 KB stages.  All copies of both CTAs
@@ -104,7 +104,10 @@ __device__ __forceinline__ void pair_arrive(uint32_t mapped_bar) {
 }
 
 // A product whose units are fewer than the pairs, or fill their last wave badly, is cut along K: a pair takes one part of a unit's K
-// blocks and parks FP32 sums, which parts_fold_kernel adds up in the order of the parts.
+// blocks and parks FP32 sums, which parts_fold_kernel adds up in the order of the parts.  The gradient of 512 x 512 weights over
+// 65536 rows is four units: 38.5 us in 18 parts of each, 58.8 with the split kernel (8 CTAs per tile of 128 x 64), whose tiles
+// read the operands twice as often (a library product: 39.7).  An instantiation of its own (PARTS): as a run-time branch it
+// cost products with short sums 5 to 10 %.
 template <typename E>
 __global__ void __launch_bounds__(256)
 parts_fold_kernel(const float* __restrict__ parts, E* __restrict__ out, int part_count, int rows, int width, int pitch, bool vectors) {
