@@ -115,6 +115,11 @@ int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const GemmGeom& g,
   auto kernel = linear_pair_kernel<E, A_MN, B_MN, PARTS>;
   static SmemAllowed allowed;
   if (int rc = allow_smem(allowed, kernel, LPR_SMEM)) return rc;
+  static const int registers = [&] {
+    cudaFuncAttributes attributes;
+    return cudaFuncGetAttributes(&attributes, kernel) == cudaSuccess ? attributes.numRegs : 0;
+  }();
+  if (registers * LPR_THREADS < LPR_REGS) return fail(I8M_E_CUDA, "%s: compiled to %d registers, too few to share out", name, registers);
   launch_clusters(kernel, 2, 2 * pairs, LPR_THREADS, LPR_SMEM, stream, ma, mb, my, mz, g, args);
   LAUNCH_CHECK(name);
   return 0;

@@ -29,9 +29,11 @@ constexpr int LPR_STAGES = 6;
 constexpr int LPR_STAGE_BYTES = 2 * TILE_BYTES;
 constexpr int LPR_EPI_WARPS = 16;
 constexpr int LPR_THREADS = 32 * (4 + LPR_EPI_WARPS);
-// 640 threads are launched with 96 registers each (65536 / 640, in eights): 61440, of which these take 60416
+// 640 threads are launched with 96 registers each (65536 / 640, in eights): 61440, of which these take 60416.  The host checks what
+// the kernel was compiled to before its first launch: with fewer, the wait for registers would not end.
 constexpr int LPR_CTRL_REGS = 56, LPR_EPI_REGS = 104;
-static_assert(32 * (4 * LPR_CTRL_REGS + LPR_EPI_WARPS * LPR_EPI_REGS) <= LPR_THREADS * (65536 / LPR_THREADS / 8 * 8), "registers");
+constexpr int LPR_REGS = 32 * (4 * LPR_CTRL_REGS + LPR_EPI_WARPS * LPR_EPI_REGS);
+static_assert(LPR_REGS <= LPR_THREADS * (65536 / LPR_THREADS / 8 * 8), "registers");
 constexpr size_t LPR_SMEM = size_t(LPR_STAGES) * LPR_STAGE_BYTES + sizeof(Ctrl) + LPR_EPI_WARPS * WARP_PATCH_BYTES + 1024;
 static_assert(LPR_SMEM <= 227 * 1024, "shared memory of a CTA");
 
