@@ -423,7 +423,8 @@ __device__ __forceinline__ void store_row_sums(const unsigned long long (&dw)[V]
 // scalar arithmetic issued 34 instructions per 32 elements' worth of work, 2.6 a cycle).  Hence: arithmetic on pairs, two sums
 // for the price of one exchange, pointers that advance instead of row * width, and a ring of rows in shared memory that each
 // thread fills for itself with asynchronous copies, 16-byte pieces of all threads side by side (with a thread's pieces
-// together, 272 bytes from its neighbour's, a pass took 109 us instead of 81).
+// together, 272 bytes from its neighbour's, a pass took 109 us instead of 81).  Twice the threads with one octet each, and so 32
+// warps per SM instead of 16, took 102 us: the exchanges of the row's sums are per warp.
 // SHIFT: rows that start anywhere, their pieces copied by all threads of the row and read behind a barrier.
 // V <= 2 keeps u and g in registers between the two sweeps; V = 4 (rows above 8192) reads them again from shared memory.
 template <typename E, bool WARP, int V, int FORMAT, bool SHIFT>

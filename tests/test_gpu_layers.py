@@ -663,3 +663,35 @@ def test_the_first_work_of_a_thread(cuda_device):
     root = pathlib.Path(__file__).resolve().parent.parent
     done = subprocess.run([sys.executable, "-c", FRESH_THREADS], cwd=root, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr
+
+
+CAPTURED_AT_FIRST = """
+import torch
+from i8muon_b200 import check_status, layer_norm, linear
+one = torch.ones(1, 8, dtype=torch.bfloat16, device="cuda")
+linear(one, one)                                   # the device's status word; no kernel of the sizes below has run
+gen = torch.Generator(device="cuda").manual_seed(1)
+def leaf(*shape, std=1.0):
+    return torch.randn(shape, device="cuda", generator=gen).mul_(std).bfloat16().requires_grad_()
+leaves = h, nw, w1, w2 = leaf(3000, 640), leaf(640), leaf(1280, 640, std=0.04), leaf(640, 1280, std=0.03)
+dy = torch.randn(3000, 640, device="cuda", generator=gen).bfloat16()
+def step():
+    y = linear(linear(layer_norm(h, nw, checkpoint="fp8"), w1, activation="silu", checkpoint="int8"), w2, residual=h)
+    return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.graph(graph, stream=side):
+    captured = step()
+graph.replay()
+torch.cuda.synchronize()
+check_status()
+for a, b in zip(captured, step()):
+    assert torch.equal(a, b)
+"""
+
+
+def test_first_calls_of_kernels_under_capture(cuda_device):
+    root = pathlib.Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", CAPTURED_AT_FIRST], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr
