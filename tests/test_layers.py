@@ -119,5 +119,8 @@ def test_native_linear_argument_errors_are_codes():
     assert backward(act=3, z=p) == -2            # dz needs room
     assert backward(outer=9) == -2               # dy's rows start anywhere: a copy
     assert backward(dx=None, db=p) == -2         # partial sums
+    assert backward(dx=None, db=p, ws=p + 16, size=1 << 20) == -1 and forward(inner=17, ws=p + 8, size=1 << 20) == -1
+    # a long sum into few tiles takes FP32 parts, up to 64 MB of them
+    assert 0 < native.linear_backward_workspace_bytes(p, p, p, 65536, 512, 512, 0, -1, 0, 1, 0) <= 64 << 20
     assert native.linear_backward_workspace_bytes(p, p, p, 4, 16, 8, 0, -1, 1, 1, 0) == 0
     assert native.linear_backward_workspace_bytes(p, p, p, 4, 16, 8, 0, 0, 0, 1, 0) >= 4 * 16 * 2
