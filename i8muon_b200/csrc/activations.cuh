@@ -75,6 +75,10 @@ __device__ __forceinline__ unsigned long long activate(unsigned long long z) {
   if constexpr (ACT == ACT_SILU) return mul2(z, gate2(mul2(z, both(-LOG2_E))));
   return z;
 }
+// z as a factor of s (1 - s), s the logistic function of z or of a cubic in it: bounded, and its square as well, so that the
+// product is zero where s is 0 or 1 to the last bit (from |z| = 90 on), at infinities too - a kept pre-activation is one where the
+// forward pass's FP32 value is beyond the kept type.  A NaN is lost here and stays in s.
+__device__ __forceinline__ float bounded_value(float z) { return fminf(fmaxf(z, -1e15f), 1e15f); }
 template <int ACT>
 __device__ __forceinline__ unsigned long long derivative(unsigned long long z) {
   const float z0 = lane0(z), z1 = lane1(z);
@@ -88,15 +92,14 @@ __device__ __forceinline__ unsigned long long derivative(unsigned long long z) {
     return fma2(mul2(b, both(0.39894228040143268f)), n.density, pair(z0 < 0.f ? t0 : 1.f - t0, z1 < 0.f ? t1 : 1.f - t1));
   }
   if constexpr (ACT == ACT_GELU_TANH) {
-    // z^2 bounded, so that the slope is finite where s (1 - s) is zero (from |z| = 10 on); a NaN stays one in z itself
-    const unsigned long long q = pair(fminf(z0 * z0, 1e30f), fminf(z1 * z1, 1e30f));
+    const unsigned long long b = pair(bounded_value(z0), bounded_value(z1)), q = mul2(b, b);
     const unsigned long long s = gate2(mul2(z, fma2(both(-LOG2_E * GELU_TANH_K), q, both(-LOG2_E * GELU_TANH_C))));
     const unsigned long long slope = fma2(both(3.f * GELU_TANH_K), q, both(GELU_TANH_C));
-    return fma2(mul2(mul2(z, s), fma2(s, both(-1.f), both(1.f))), slope, s);
+    return fma2(mul2(mul2(b, s), fma2(s, both(-1.f), both(1.f))), slope, s);
   }
   if constexpr (ACT == ACT_SILU) {
-    const unsigned long long s = gate2(mul2(z, both(-LOG2_E)));
-    return fma2(mul2(z, s), fma2(s, both(-1.f), both(1.f)), s);
+    const unsigned long long s = gate2(mul2(z, both(-LOG2_E))), b = pair(bounded_value(z0), bounded_value(z1));
+    return fma2(mul2(b, s), fma2(s, both(-1.f), both(1.f)), s);
   }
   return both(1.f);
 }
