@@ -120,24 +120,24 @@ int linear_dz(const LinearDz& d, cudaStream_t stream) {
 }  // namespace i8m
 
 // ================================================================== eight-bit activations
-static int check_eight(const char* name, const void* a, const void* codes, const void* exponents, long long rows, int width,
+static int check_eight(const char* name, const void* a, const void* codes, const void* exponents, long long rows, long long width,
                        int dtype, int format) {
   if (!a || !codes || !exponents) return fail(I8M_E_ARGUMENT, "%s: null pointer", name);
   if (rows < 1 || width < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
   if (!float_dtype_ok(dtype)) return fail(I8M_E_ARGUMENT, "%s: bad dtype %d", name, dtype);
   if (format != EIGHT_INT8 && format != EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
   if (reinterpret_cast<uintptr_t>(codes) & 15u) return fail(I8M_E_ARGUMENT, "%s: codes are not 16-byte aligned", name);
-  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %d is above %d", name, width, MAX_LAYER_WIDTH);
+  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %lld is above %d", name, width, MAX_LAYER_WIDTH);
   if (rows > MAX_LAYER_ROWS) return fail(I8M_E_LIMIT, "%s: %lld rows are above %lld", name, rows, MAX_LAYER_ROWS);
   return 0;
 }
-extern "C" int i8m_activation_quant(const void* x, int dtype, long long rows, int width, int format, void* codes,
+extern "C" int i8m_activation_quant(const void* x, int dtype, long long rows, long long width, int format, void* codes,
                                     void* exponents, i8m_stream_t stream) {
   if (int rc = check_eight("activation_quant", x, codes, exponents, rows, width, dtype, format)) return rc;
-  return eight_quant(x, dtype, rows, width, format, codes, exponents, S(stream));
+  return eight_quant(x, dtype, rows, int(width), format, codes, exponents, S(stream));
 }
-extern "C" int i8m_activation_restore(const void* codes, const void* exponents, long long rows, int width, int format,
+extern "C" int i8m_activation_restore(const void* codes, const void* exponents, long long rows, long long width, int format,
                                       void* out, int dtype, i8m_stream_t stream) {
   if (int rc = check_eight("activation_restore", out, codes, exponents, rows, width, dtype, format)) return rc;
-  return eight_restore(codes, exponents, rows, width, format, out, dtype, width, S(stream));
+  return eight_restore(codes, exponents, rows, int(width), format, out, dtype, int(width), S(stream));
 }

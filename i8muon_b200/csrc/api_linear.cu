@@ -166,13 +166,14 @@ int product_of(int dtype, A&&... args) {
   return dtype == I8M_F16 ? product<__half>(std::forward<A>(args)...) : product<__nv_bfloat16>(std::forward<A>(args)...);
 }
 
-int check_linear(const char* name, int rows, int inner, int outer, int dtype, int activation, int format) {
+// Extents come as 64-bit numbers: what a caller passes is what is compared with the limits.
+int check_linear(const char* name, long long rows, long long inner, long long outer, int dtype, int activation, int format) {
   if (rows < 1 || inner < 1 || outer < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
   if (dtype != I8M_F16 && dtype != I8M_BF16) return fail(I8M_E_ARGUMENT, "%s: dtype must be a 16-bit type", name);
   if (activation < 0 || activation >= ACTIVATIONS) return fail(I8M_E_ARGUMENT, "%s: bad activation %d", name, activation);
   if (format < -1 || format > EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
   if (inner > MAX_LAYER_WIDTH || outer > MAX_LAYER_WIDTH || rows > MAX_LAYER_ROWS)
-    return fail(I8M_E_LIMIT, "%s: %d rows, %d x %d weights are above the limits", name, rows, outer, inner);
+    return fail(I8M_E_LIMIT, "%s: %lld rows, %lld x %lld weights are above the limits", name, rows, outer, inner);
   return 0;
 }
 
@@ -226,17 +227,20 @@ struct BackwardPieces {
 
 }  // namespace
 
-extern "C" int i8m_linear_workspace_bytes(const void* x, const void* weight, int rows, int inner, int outer, size_t* bytes) {
+extern "C" int i8m_linear_workspace_bytes(const void* x, const void* weight, long long rows, long long inner, long long outer,
+                                          size_t* bytes) {
   if (!bytes) return fail(I8M_E_ARGUMENT, "linear_workspace_bytes: null pointer");
   if (int rc = check_linear("linear_workspace_bytes", rows, inner, outer, I8M_BF16, 0, -1)) return rc;
-  *bytes = ForwardPieces(nullptr, x, weight, rows, inner, outer).bytes;
+  *bytes = ForwardPieces(nullptr, x, weight, int(rows), int(inner), int(outer)).bytes;
   return 0;
 }
 extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z,
-                          void* z_codes, void* z_exponents, int format, int activation, int rows, int inner, int outer, int dtype,
-                          void* workspace, size_t workspace_bytes, uint32_t* status, i8m_stream_t stream) {
+                          void* z_codes, void* z_exponents, int format, int activation, long long row_count, long long inner_width,
+                          long long outer_width, int dtype, void* workspace, size_t workspace_bytes, uint32_t* status,
+                          i8m_stream_t stream) {
   if (!x || !weight || !y || !status) return fail(I8M_E_ARGUMENT, "linear: null pointer");
-  if (int rc = check_linear("linear", rows, inner, outer, dtype, activation, format)) return rc;
+  if (int rc = check_linear("linear", row_count, inner_width, outer_width, dtype, activation, format)) return rc;
+  const int rows = int(row_count), inner = int(inner_width), outer = int(outer_width);
   if (format >= 0 && !z_codes != !z_exponents) return fail(I8M_E_ARGUMENT, "linear: codes without exponents");
   if ((reinterpret_cast<uintptr_t>(z) | (format >= 0 ? reinterpret_cast<uintptr_t>(z_codes) : 0)) & 15u)
     return fail(I8M_E_ARGUMENT, "linear: z or its codes are not 16-byte aligned");
@@ -255,19 +259,22 @@ extern "C" int i8m_linear(const void* x, const void* weight, const void* bias, c
                     inner, a, nullptr, size_t(0), status, S(stream), "linear");
 }
 
-extern "C" int i8m_linear_backward_workspace_bytes(const void* dy, const void* x, const void* weight, int rows, int inner, int outer,
-                                                   int activation, int format, int dx, int dweight, int dbias, size_t* bytes) {
+extern "C" int i8m_linear_backward_workspace_bytes(const void* dy, const void* x, const void* weight, long long rows, long long inner,
+                                                   long long outer, int activation, int format, int dx, int dweight, int dbias,
+                                                   size_t* bytes) {
   if (!bytes) return fail(I8M_E_ARGUMENT, "linear_backward_workspace_bytes: null pointer");
   if (int rc = check_linear("linear_backward_workspace_bytes", rows, inner, outer, I8M_BF16, activation, format)) return rc;
-  *bytes = BackwardPieces(nullptr, dy, x, weight, rows, inner, outer, activation, format, dx, dweight, dbias).bytes;
+  *bytes = BackwardPieces(nullptr, dy, x, weight, int(rows), int(inner), int(outer), activation, format, dx, dweight, dbias).bytes;
   return 0;
 }
 extern "C" int i8m_linear_backward(const void* dy, const void* x, const void* x_codes, const void* x_exponents, const void* weight,
                                    const void* z, const void* z_codes, const void* z_exponents, int format, int activation,
-                                   void* dx, void* dweight, void* dbias, int rows, int inner, int outer, int dtype,
-                                   void* workspace, size_t workspace_bytes, uint32_t* status, i8m_stream_t stream) {
+                                   void* dx, void* dweight, void* dbias, long long row_count, long long inner_width,
+                                   long long outer_width, int dtype, void* workspace, size_t workspace_bytes, uint32_t* status,
+                                   i8m_stream_t stream) {
   if (!dy || !status || (!dx && !dweight && !dbias)) return fail(I8M_E_ARGUMENT, "linear_backward: null pointer");
-  if (int rc = check_linear("linear_backward", rows, inner, outer, dtype, activation, format)) return rc;
+  if (int rc = check_linear("linear_backward", row_count, inner_width, outer_width, dtype, activation, format)) return rc;
+  const int rows = int(row_count), inner = int(inner_width), outer = int(outer_width);
   if (dx && !weight) return fail(I8M_E_ARGUMENT, "linear_backward: dx needs the weight");
   if (dweight && (format < 0 ? !x : !x_codes || !x_exponents))
     return fail(I8M_E_ARGUMENT, "linear_backward: the weight's gradient needs x or its codes");

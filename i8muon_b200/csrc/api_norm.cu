@@ -10,7 +10,7 @@ using namespace i8m;
 // ================================================================== layer norm
 namespace {
 
-int check_norm(const char* name, const void* a, const void* b, long long rows, int width, int dtype, const void* codes,
+int check_norm(const char* name, const void* a, const void* b, long long rows, long long width, int dtype, const void* codes,
                const void* exponents, int format) {
   if (!a || !b) return fail(I8M_E_ARGUMENT, "%s: null pointer", name);
   if (rows < 1 || width < 1) return fail(I8M_E_ARGUMENT, "%s: empty problem", name);
@@ -18,7 +18,7 @@ int check_norm(const char* name, const void* a, const void* b, long long rows, i
   if (format < -1 || format > EIGHT_E4M3) return fail(I8M_E_ARGUMENT, "%s: bad format %d", name, format);
   if (format >= 0 && (!codes || !exponents)) return fail(I8M_E_ARGUMENT, "%s: null codes or exponents", name);
   if (format >= 0 && (reinterpret_cast<uintptr_t>(codes) & 15u)) return fail(I8M_E_ARGUMENT, "%s: codes are not 16-byte aligned", name);
-  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %d is above %d", name, width, MAX_LAYER_WIDTH);
+  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "%s: width %lld is above %d", name, width, MAX_LAYER_WIDTH);
   if (rows > MAX_LAYER_ROWS) return fail(I8M_E_LIMIT, "%s: %lld rows are above %lld", name, rows, MAX_LAYER_ROWS);
   return 0;
 }
@@ -51,9 +51,10 @@ bool ln_vectors(int width, std::initializer_list<const void*> tensors) {
 }  // namespace
 
 extern "C" int i8m_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
-                              void* codes, void* exponents, int format, long long rows, int width, int dtype, float eps,
+                              void* codes, void* exponents, int format, long long rows, long long row_width, int dtype, float eps,
                               i8m_stream_t stream) {
-  if (int rc = check_norm("layer_norm", x, y, rows, width, dtype, codes, exponents, format)) return rc;
+  if (int rc = check_norm("layer_norm", x, y, rows, row_width, dtype, codes, exponents, format)) return rc;
+  const int width = int(row_width);
   const int groups = eight_groups(width);
   const LnShape shape = ln_shape(width, LN_FORWARD_OCTETS);
   uint8_t *c = static_cast<uint8_t*>(codes), *e = static_cast<uint8_t*>(exponents);
@@ -85,17 +86,18 @@ extern "C" int i8m_layer_norm(const void* x, const void* weight, const void* bia
   return 0;
 }
 
-extern "C" int i8m_layer_norm_scratch_bytes(long long rows, int width, size_t* bytes) {
+extern "C" int i8m_layer_norm_scratch_bytes(long long rows, long long width, size_t* bytes) {
   if (rows < 1 || width < 1 || !bytes) return fail(I8M_E_ARGUMENT, "layer_norm_scratch_bytes: bad argument");
-  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "layer_norm_scratch_bytes: width %d is above %d", width, MAX_LAYER_WIDTH);
-  *bytes = size_t(ln_bands(rows, width)) * 2 * size_t(width) * sizeof(float);
+  if (width > MAX_LAYER_WIDTH) return fail(I8M_E_LIMIT, "layer_norm_scratch_bytes: width %lld is above %d", width, MAX_LAYER_WIDTH);
+  *bytes = size_t(ln_bands(rows, int(width))) * 2 * size_t(width) * sizeof(float);
   return 0;
 }
 extern "C" int i8m_layer_norm_backward(const void* dy, const void* x, const float* mean, const float* rstd, const void* codes,
                                        const void* exponents, int format, const void* weight, void* dx, void* dweight,
-                                       void* dbias, long long rows, int width, int dtype, void* scratch, size_t scratch_bytes,
-                                       i8m_stream_t stream) {
-  if (int rc = check_norm("layer_norm_backward", dy, rstd, rows, width, dtype, codes, exponents, format)) return rc;
+                                       void* dbias, long long rows, long long row_width, int dtype, void* scratch,
+                                       size_t scratch_bytes, i8m_stream_t stream) {
+  if (int rc = check_norm("layer_norm_backward", dy, rstd, rows, row_width, dtype, codes, exponents, format)) return rc;
+  const int width = int(row_width);
   if (format < 0 && (!x || !mean)) return fail(I8M_E_ARGUMENT, "layer_norm_backward: neither x and its means nor codes");
   if (!dx && !dweight && !dbias) return fail(I8M_E_ARGUMENT, "layer_norm_backward: nothing to compute");
   size_t need = 0;

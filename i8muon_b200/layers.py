@@ -28,6 +28,7 @@ GROUP = 32
 _FORMATS = {None: native.EIGHT_NONE, "int8": native.EIGHT_INT8, "fp8": native.EIGHT_E4M3}
 _CODE_TYPES = {native.EIGHT_INT8: torch.int8, native.EIGHT_E4M3: torch.float8_e4m3fn}
 _ACTIVATIONS = {None: 0, "relu": 1, "relu2": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
+_MOST_WIDTH, _MOST_ROWS = native.MAX_LAYER_WIDTH, native.MAX_LAYER_ROWS
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -73,7 +74,14 @@ def _check_rows(function, x, dtypes=_FLOATS):
     width = x.shape[-1]
     if width < 1:
         raise ValueError(f"{function}: the last dimension must not be empty")
-    return x.numel() // width, width
+    rows = x.numel() // width
+    if width > _MOST_WIDTH or rows > _MOST_ROWS:
+        raise _too_large(function, rows, width)
+    return rows, width
+
+
+def _too_large(function, rows, width):
+    return ValueError(f"{function}: {rows} rows of {width} elements are above the limits, {_MOST_ROWS} rows and {_MOST_WIDTH} elements")
 
 
 def _check_vector(function, name, v, width, dtype):
@@ -156,6 +164,9 @@ def restore_activation(q: QuantisedActivation) -> Tensor:
     if (q.codes.shape != (*shape[:-1], groups * GROUP) or q.codes.dtype != _CODE_TYPES[fmt]
             or q.exponents.shape != (*shape[:-1], groups) or q.exponents.dtype != torch.uint8):
         raise ValueError("restore_activation: codes and exponents do not belong to a tensor of this shape")
+    rows = q.exponents.numel() // groups
+    if width > _MOST_WIDTH or rows > _MOST_ROWS:
+        raise _too_large("restore_activation", rows, width)
     _check_device("restore_activation", q.codes, q.exponents)
     device = q.codes.device
     codes, exponents = q.codes.contiguous(), q.exponents.contiguous()
@@ -163,8 +174,8 @@ def restore_activation(q: QuantisedActivation) -> Tensor:
         codes = codes.clone()
     with on_device(device.index):
         out = codes.new_empty(shape, dtype=q.dtype)
-        if out.numel():
-            native.call("i8m_activation_restore", codes.data_ptr(), exponents.data_ptr(), out.numel() // width, width, fmt,
+        if rows:
+            native.call("i8m_activation_restore", codes.data_ptr(), exponents.data_ptr(), rows, width, fmt,
                         out.data_ptr(), native.torch_dtype_code(q.dtype), raw_stream(device.index))
     return out
 
@@ -401,6 +412,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     if not isinstance(weight, Tensor) or weight.ndim != 2 or weight.shape[1] != inner or weight.dtype != x.dtype or weight.shape[0] < 1:
         raise ValueError(f"linear: weight must be a matrix of {inner} columns of the input's type")
     outer = weight.shape[0]
+    if outer > _MOST_WIDTH:
+        raise _too_large("linear", outer, inner)
     _check_vector("linear", "bias", bias, outer, x.dtype)
     if residual is not None and (not isinstance(residual, Tensor) or residual.shape != (*x.shape[:-1], outer)
                                  or residual.dtype != x.dtype):

@@ -16,6 +16,7 @@ from .build import LIBRARY
 
 F32, F16, BF16 = 0, 1, 2
 EIGHT_NONE, EIGHT_INT8, EIGHT_E4M3 = -1, 0, 1
+MAX_LAYER_WIDTH, MAX_LAYER_ROWS = 1 << 24, (1 << 31) - 1 - 1024     # csrc/layers.cuh
 ROUTE_FLOAT, ROUTE_GRAM, ROUTE_INT8, ROUTE_BQ_INT8, ROUTE_BQ_FP8, ROUTE_INT8_FACTORED, ROUTE_INT8_CUBIC = range(7)
 
 
@@ -78,18 +79,20 @@ _SIGNATURES = {
                                c_float, c_float, _P]),
     "i8m_adamw": (c_int, [POINTER(_P), POINTER(_P), POINTER(_P), POINTER(_P), POINTER(c_longlong), c_int,
                           c_int, c_int, c_float, c_float, c_float, c_float, c_float, c_float, c_float, _P]),
-    "i8m_activation_quant": (c_int, [_P, c_int, c_longlong, c_int, c_int, _P, _P, _P]),
-    "i8m_activation_restore": (c_int, [_P, _P, c_longlong, c_int, c_int, _P, c_int, _P]),
-    "i8m_layer_norm": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_longlong, c_int, c_int, c_float, _P]),
-    "i8m_layer_norm_scratch_bytes": (c_int, [c_longlong, c_int, POINTER(c_size_t)]),
-    "i8m_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, _P, c_longlong, c_int, c_int, _P, c_size_t,
-                                        _P]),
-    "i8m_linear_workspace_bytes": (c_int, [_P, _P, c_int, c_int, c_int, POINTER(c_size_t)]),
-    "i8m_linear": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
-    "i8m_linear_backward_workspace_bytes": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
-                                                    POINTER(c_size_t)]),
-    "i8m_linear_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, _P,
-                                    c_size_t, _P, _P]),
+    # extents of the layers are 64-bit: ctypes drops the high bits of what is passed as a c_int without an error
+    "i8m_activation_quant": (c_int, [_P, c_int, c_longlong, c_longlong, c_int, _P, _P, _P]),
+    "i8m_activation_restore": (c_int, [_P, _P, c_longlong, c_longlong, c_int, _P, c_int, _P]),
+    "i8m_layer_norm": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_longlong, c_longlong, c_int, c_float, _P]),
+    "i8m_layer_norm_scratch_bytes": (c_int, [c_longlong, c_longlong, POINTER(c_size_t)]),
+    "i8m_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, _P, c_longlong, c_longlong, c_int, _P,
+                                        c_size_t, _P]),
+    "i8m_linear_workspace_bytes": (c_int, [_P, _P, c_longlong, c_longlong, c_longlong, POINTER(c_size_t)]),
+    "i8m_linear": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_longlong, c_longlong, c_longlong, c_int, _P, c_size_t,
+                           _P, _P]),
+    "i8m_linear_backward_workspace_bytes": (c_int, [_P, _P, _P, c_longlong, c_longlong, c_longlong, c_int, c_int, c_int, c_int,
+                                                    c_int, POINTER(c_size_t)]),
+    "i8m_linear_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, c_longlong, c_longlong, c_longlong,
+                                    c_int, _P, c_size_t, _P, _P]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

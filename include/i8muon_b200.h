@@ -280,11 +280,12 @@ int i8m_adamw(void* const* params, const void* const* grads, float* const* exp_a
  *   codes      rows x 32 ceil(width / 32) bytes, zero behind the width; 16-byte aligned
  *   exponents  rows x ceil(width / 32) bytes e + 127; 255 marks a group that holds an infinity or a NaN and reads back as
  *              NaN throughout
+ * Limits of the layers: 2^24 elements of a row (inner, outer, width) and 2^31 - 1025 rows; more is I8M_E_LIMIT.
  * `format` of these functions is an i8m_eight_format; where it may be I8M_EIGHT_NONE the codes are not used. */
 enum i8m_eight_format { I8M_EIGHT_NONE = -1, I8M_EIGHT_INT8 = 0, I8M_EIGHT_E4M3 = 1 };
-int i8m_activation_quant(const void* x_device, int dtype, long long rows, int width, int format, void* codes_device,
+int i8m_activation_quant(const void* x_device, int dtype, long long rows, long long width, int format, void* codes_device,
                          void* exponents_device, i8m_stream_t stream);
-int i8m_activation_restore(const void* codes_device, const void* exponents_device, long long rows, int width, int format,
+int i8m_activation_restore(const void* codes_device, const void* exponents_device, long long rows, long long width, int format,
                            void* out_device, int dtype, i8m_stream_t stream);
 
 /* Layer norm over rows of `width` elements: u = (x - mean) rstd, rstd = 1 / sqrt(var + eps), y = u * weight + bias, all in
@@ -292,14 +293,14 @@ int i8m_activation_restore(const void* codes_device, const void* exponents_devic
  * weight, bias: NULL = ones, zeros.  mean, rstd: FP32 [rows] for the backward pass, or NULL.  format: I8M_EIGHT_NONE, or u is
  * also written in eight bits (codes, exponents), which then serve the backward pass in the place of x and mean. */
 int i8m_layer_norm(const void* x_device, const void* weight_device, const void* bias_device, void* y_device, float* mean_device,
-                   float* rstd_device, void* codes_device, void* exponents_device, int format, long long rows, int width,
+                   float* rstd_device, void* codes_device, void* exponents_device, int format, long long rows, long long width,
                    int dtype, float eps, i8m_stream_t stream);
 /* Gradients of the above; dx, dweight, dbias may each be NULL.  scratch (only for dweight and dbias): partial sums over
  * bands of rows, added up in a fixed order. */
-int i8m_layer_norm_scratch_bytes(long long rows, int width, size_t* bytes);
+int i8m_layer_norm_scratch_bytes(long long rows, long long width, size_t* bytes);
 int i8m_layer_norm_backward(const void* dy_device, const void* x_device, const float* mean_device, const float* rstd_device,
                             const void* codes_device, const void* exponents_device, int format, const void* weight_device,
-                            void* dx_device, void* dweight_device, void* dbias_device, long long rows, int width, int dtype,
+                            void* dx_device, void* dweight_device, void* dbias_device, long long rows, long long width, int dtype,
                             void* scratch_device, size_t scratch_bytes, i8m_stream_t stream);
 
 /* Linear layer: z = x weight^T + bias, y = act(z) + residual, sums in FP32, y rounded once to `dtype` (I8M_F16 or I8M_BF16:
@@ -312,22 +313,23 @@ enum i8m_activation {
   I8M_ACT_NONE = 0, I8M_ACT_RELU = 1, I8M_ACT_RELU2 = 2 /* max(z, 0)^2 */, I8M_ACT_GELU = 3 /* z Phi(z) */,
   I8M_ACT_GELU_TANH = 4, I8M_ACT_SILU = 5
 };
-int i8m_linear_workspace_bytes(const void* x_device, const void* weight_device, int rows, int inner, int outer, size_t* bytes);
+int i8m_linear_workspace_bytes(const void* x_device, const void* weight_device, long long rows, long long inner, long long outer,
+                               size_t* bytes);
 int i8m_linear(const void* x_device, const void* weight_device, const void* bias_device, const void* residual_device,
                void* y_device, void* z_device, void* z_codes_device, void* z_exponents_device, int format, int activation,
-               int rows, int inner, int outer, int dtype, void* workspace_device, size_t workspace_bytes,
+               long long rows, long long inner, long long outer, int dtype, void* workspace_device, size_t workspace_bytes,
                uint32_t* status_device, i8m_stream_t stream);
 /* Gradients of the above (the residual's is dy itself); dx, dweight, dbias may each be NULL.  dz = dy act'(z) at the kept z,
  * rounded to `dtype` as the operand of dx = dz weight and dweight = dz^T x; dbias sums the unrounded dz over bands of rows in
  * a fixed order.  x, or its codes (i8m_activation_quant) where `format` names a format, serves dweight; z or its codes serve an
  * activation.  dx, dweight and dbias in the arguments of the query are truth values.  workspace (32-byte aligned): dz, copies as
  * above, bands of dbias, and up to 64 MB of FP32 parts where a gradient is a long sum into few tiles. */
-int i8m_linear_backward_workspace_bytes(const void* dy_device, const void* x_device, const void* weight_device, int rows, int inner,
-                                        int outer, int activation, int format, int dx, int dweight, int dbias, size_t* bytes);
+int i8m_linear_backward_workspace_bytes(const void* dy_device, const void* x_device, const void* weight_device, long long rows,
+                                        long long inner, long long outer, int activation, int format, int dx, int dweight, int dbias, size_t* bytes);
 int i8m_linear_backward(const void* dy_device, const void* x_device, const void* x_codes_device, const void* x_exponents_device,
                         const void* weight_device, const void* z_device, const void* z_codes_device,
                         const void* z_exponents_device, int format, int activation, void* dx_device, void* dweight_device,
-                        void* dbias_device, int rows, int inner, int outer, int dtype, void* workspace_device,
+                        void* dbias_device, long long rows, long long inner, long long outer, int dtype, void* workspace_device,
                         size_t workspace_bytes, uint32_t* status_device, i8m_stream_t stream);
 
 #ifdef __cplusplus
