@@ -2,8 +2,8 @@
 
 ``linear`` (bias, activation and residual in the product's epilogue), ``layer_norm``, and activations kept in eight bits for the backward pass (``quantise_activation``, ``restore_activation``,
 and the ``checkpoint=`` argument of the layers).  The functions take and return torch tensors, work on
-the current stream of the tensors' device without synchronising, and are differentiable once.  They run the sm_100a library's
-kernels; there is no fallback.  The reference starts at the gradient and has no counterpart.
+the current stream of the tensors' device without synchronising, and are differentiable once, in reverse mode; tensors that
+carry a tangent of forward mode are refused.  They run the sm_100a library's kernels; there is no fallback.  The reference starts at the gradient and has no counterpart.
 
 Eight-bit format: groups of 32 consecutive elements of a row share a power of two, the smallest 2^e with
 max|x| <= M 2^e (M = 127 for ``"int8"``, 448 for ``"fp8"``, E4M3; e >= -127), and each element is rounded to the nearest
@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import native
@@ -117,6 +118,15 @@ def _any_gradient(*tensors) -> bool:
     return False
 
 
+def _refuse_tangents(function, *tensors):
+    """A dual tensor of forward mode need not require a gradient, and the kernels would drop its tangent: a derivative of zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # no level is entered, which is nearly always
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{function} has no forward-mode derivative")
+
+
 # ------------------------------------------------------- activations in eight bits
 def _quantise(x, rows, width, fmt, codes_at, exponents_at):
     """A contiguous ``x`` to codes and exponents at two addresses; its device must be current."""
@@ -137,6 +147,7 @@ def quantise_activation(x: Tensor, checkpoint: str = "int8") -> QuantisedActivat
     if fmt == native.EIGHT_NONE:
         raise ValueError("quantise_activation: checkpoint must be 'int8' or 'fp8'")
     rows, width = _check_rows("quantise_activation", x)
+    _refuse_tangents("quantise_activation", x)
     _check_device("quantise_activation", x)
     groups = -(-width // GROUP)
     shape = x.shape
@@ -233,6 +244,7 @@ def _norm_backward(ctx, dy):
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     fmt, shape, offset = ctx.settings
     kept, stats, *weight = ctx.saved_tensors
+    _refuse_tangents("layer_norm", dy)
     width = shape[-1]
     dy = dy.contiguous()
     rows, index = dy.numel() // width, dy.device.index
@@ -273,6 +285,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError("layer_norm: eps must be >= 0")
+    _refuse_tangents("layer_norm", x, weight, bias)
     _check_device("layer_norm", x, weight, bias)
     if _any_gradient(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps, fmt)
@@ -354,6 +367,7 @@ class _Linear(torch.autograd.Function):
 def _linear_backward(ctx, dy):
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     activation, fmt, x_shape, w_shape, kept_z, x_offset, z_offset = ctx.settings
+    _refuse_tangents("linear", dy)
     dresidual = dy if need_r else None
     if not (need_x or need_w or need_b):
         return None, None, None, dresidual, None, None
@@ -418,6 +432,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     if residual is not None and (not isinstance(residual, Tensor) or residual.shape != (*x.shape[:-1], outer)
                                  or residual.dtype != x.dtype):
         raise ValueError("linear: residual must have the shape and type of the result")
+    _refuse_tangents("linear", x, weight, bias, residual)
     _check_device("linear", x, weight, bias, residual)
     if _any_gradient(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, _ACTIVATIONS[activation], fmt)
