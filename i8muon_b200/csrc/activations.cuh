@@ -8,7 +8,8 @@ namespace i8m {
 enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_RELU2 = 2, ACT_GELU = 3, ACT_GELU_TANH = 4, ACT_SILU = 5 };
 constexpr int ACTIVATIONS = 6;
 
-// 2^v and 1 / v on the special-function unit, good to a few units in the last place; 1 / inf is 0.
+// 2^v and 1 / v on the special-function unit, good to a few units in the last place; 1 / inf is 0, and results below 2^-126
+// are 0: silu below z = -87.3, where its value is -1e-36, and gelu_tanh below -10.0, where it is -1.2e-37.
 __device__ __forceinline__ float exp2_fast(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -29,8 +30,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays
 
 // Normal distribution: the lower tail Phi(-a) and exp(-a^2 / 2) for two a = min(|z|, 30) (beyond 14 the tail is zero in FP32).
 // With t = 1 / (1 + 0.3 a), Phi(-a) is exp(-a^2 / 2) t P(t): Phi(-a) exp(a^2 / 2) falls like 1 / a, so it is t times a smooth
-// function, here a polynomial of degree 7 fitted for the least relative error over 0 <= a <= 14: 1.5e-7 in exact arithmetic,
-// 5e-7 with FP32 roundings over a grid of 200 000 points.  Ten issue slots per element with the pairs, twenty without.
+// function, here a polynomial of degree 7 fitted for the least relative error over 0 <= a <= 14: t P(t) is good to 1.5e-7 in
+// exact arithmetic and 5e-7 with FP32 roundings, over a grid of 400 000 points.  The exponential adds the roundings of its
+// argument, which grow with a^2 / 2: the tail's relative error is 6e-7 up to a = 3, 2e-6 up to 6, 3.3e-6 up to 9 and 8e-6 up to
+// 12.9, where the tail is 2e-38.  Ten issue slots per element with the pairs, twenty without.
 struct NormalTail { unsigned long long tail, density; };
 __device__ __forceinline__ NormalTail normal_tail(unsigned long long a) {
   const unsigned long long s = mul2(mul2(a, both(-0.5f * LOG2_E)), a), q = fma2(both(0.3f), a, both(1.f));

@@ -1,7 +1,10 @@
 """The layer operators where values leave a type or a range."""
+import math
+
 import pytest
 import torch
 
+import layer_reference as ref
 from i8muon_b200 import check_status, linear
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +45,50 @@ def test_slopes_at_a_pre_activation_beyond_its_type(cuda_device, beyond, outer, 
     assert torch.equal(dx.double(), dz @ w.detach().double())
     assert torch.equal(dw.double(), dz.t() @ x.detach().double())
     assert torch.equal(db.double(), dz.sum(0))
+
+
+EPS, FLUSH = 2.0 ** -24, 2.0 ** -126
+# the exponential's instruction is good to 2^-22 of its result, the reciprocal's to 2^-23; results below 2^-126 become zero
+EX2, RCP = 4 * EPS, 2 * EPS
+
+
+def activation_in_double(z, act):
+    """(value, slope, what FP32 may lose of either) in 64 bits; the lower tail of the normal distribution from erfc, which does
+    not cancel."""
+    a = z.abs()
+    if act == "gelu":
+        tail, density = 0.5 * torch.erfc(a / math.sqrt(2)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        # exponent -a^2 / 2: a constant and two products, each rounded; the polynomial's 5e-7 holds a reciprocal and FP32 sums
+        exponential = 3 * EPS * z * z / 2 + EX2
+        lost = exponential + 5e-7 + 2 * EPS
+        cdf = torch.where(z < 0, tail, 1 - tail)
+        return (z * cdf, cdf + z * density, lost * a * tail + FLUSH * a,
+                lost * tail + (exponential + 4 * EPS) * a * density + 2 * EPS * cdf + FLUSH * (1 + a))
+    if act == "silu":
+        v, dv, loss = z, torch.ones_like(z), 2 * EPS * a
+    else:
+        c = 2 * math.sqrt(2 / math.pi)
+        v, dv = c * (z + 0.044715 * z ** 3), c * (1 + 3 * 0.044715 * z * z)
+        loss = 6 * EPS * v.abs()               # two constants, a square, a cubic and the product with z
+    s, rest = torch.sigmoid(v), torch.sigmoid(-v)
+    off = s * rest * (loss + EX2) + s * (RCP + EPS) + FLUSH
+    y, slope = z * s, s + z * dv * s * rest
+    return y, slope, a * off + EPS * y.abs(), off * (1 + a * dv) + 8 * EPS * (s + a * dv * s * rest)
+
+
+@pytest.mark.parametrize("act, far", [("gelu", 12.9), ("gelu_tanh", 12.0), ("silu", 100.0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_activations_and_slopes_over_their_tails(cuda_device, act, far, dtype):
+    """z is the bias alone, every number of the type up to ``far`` (of FP16 every third): relative to the value, also where
+    that is 1e-37."""
+    bits = torch.arange(0, 1 << 15, dtype=torch.int32).to(torch.int16)
+    z = bits.view(dtype)
+    z = z[torch.isfinite(z) & (z <= far) & (z >= 2.0 ** -12)][::1 if dtype == torch.bfloat16 else 3]
+    z = torch.cat((z, -z)).to(cuda_device).requires_grad_()
+    x, w = torch.zeros(1, 8, dtype=dtype, device=cuda_device), torch.zeros(z.numel(), 8, dtype=dtype, device=cuda_device)
+    y = linear(x, w, z, activation=act)
+    got, = torch.autograd.grad(y, z, torch.ones_like(y))
+    check_status()
+    want, slope, off, off_slope = activation_in_double(z.detach().double(), act)
+    ref.assert_within(y[0].detach(), want, off + ref.half_step(want.abs() + off, dtype), "value")
+    ref.assert_within(got, slope, off_slope + ref.half_step(slope.abs() + off_slope, dtype), "slope")
