@@ -81,7 +81,13 @@ __device__ __forceinline__ unsigned long long activate(unsigned long long z) {
 // z as a factor of s (1 - s), s the logistic function of z or of a cubic in it: bounded, and its square as well, so that the
 // product is zero where s is 0 or 1 to the last bit (from |z| = 90 on), at infinities too - a kept pre-activation is one where the
 // forward pass's FP32 value is beyond the kept type.  A NaN is lost here and stays in s.
-__device__ __forceinline__ float bounded_value(float z) { return fminf(fmaxf(z, -1e15f), 1e15f); }
+// One instruction, the smaller magnitude under the product of both signs: silu's slopes for the bias gradient of 8192 x 14336
+// take 89.6 us, 91.6 with a minimum and a maximum, 88.5 without a bound; gelu_tanh's 99.4, 101.4, 98.6.
+__device__ __forceinline__ float bounded_value(float z) {
+  float r;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(1e15f));
+  return r;
+}
 template <int ACT>
 __device__ __forceinline__ unsigned long long derivative(unsigned long long z) {
   const float z0 = lane0(z), z1 = lane1(z);
