@@ -106,7 +106,7 @@ int make_block_map(CUtensorMap* map, void* ptr, int width, int rows, int pitch) 
 }  // namespace i8m
 
 // =========================================================== library state
-extern "C" int i8m_version(void) { return 100; }
+extern "C" int i8m_version(void) { return 101; }
 extern "C" const char* i8m_build_info(void) {
   static char info[256];
   snprintf(info, sizeof(info),

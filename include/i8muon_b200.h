@@ -55,6 +55,7 @@ enum i8m_route {
 };
 
 /* ---- library state ------------------------------------------------------ */
+/* 101: extents of the layers are 64-bit; a caller that was compiled against 100 and calls them has to be compiled again */
 int i8m_version(void);
 /* "arch=sm_100a cuda=<ver> tile=128x128 ..." ; static storage */
 const char* i8m_build_info(void);

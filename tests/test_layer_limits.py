@@ -77,3 +77,27 @@ def test_the_c_abi_sees_the_extents_that_were_passed():
     # what is not above the limits is asked for in full
     assert native.linear_workspace_bytes(p, p, 1 << 30, 17, 8) >= (1 << 30) * 24 * 2
     assert native.layer_norm_scratch_bytes(4, native.MAX_LAYER_WIDTH) == 4 * 2 * native.MAX_LAYER_WIDTH * 4
+
+
+def test_every_extent_is_bound_as_a_64_bit_number():
+    """The header's parameters and the binding's, one by one: an int here and a long long there would pass garbage."""
+    import re
+    from ctypes import c_float, c_int, c_longlong, c_size_t
+    from pathlib import Path
+    text = (Path(__file__).resolve().parents[1] / "include" / "i8muon_b200.h").read_text()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    scalars = {"int": c_int, "long long": c_longlong, "float": c_float, "size_t": c_size_t}
+    names = [n for n in native.EXPORTED_SYMBOLS if n.startswith(("i8m_linear", "i8m_layer_norm", "i8m_activation"))]
+    assert len(names) == 9 and native.library().i8m_version() >= 101
+    for name in names:
+        declared = re.search(rf"\bint {name}\(([^)]*)\)", text).group(1).split(",")
+        bound = native._SIGNATURES[name][1]
+        assert len(declared) == len(bound), name
+        for parameter, kind in zip(declared, bound):
+            words = parameter.split()
+            if "*" in parameter or words[0] == "i8m_stream_t":
+                assert kind not in scalars.values(), (name, parameter)
+            else:
+                assert kind is scalars[" ".join(words[:-1])], (name, parameter)
+                if words[-1] in ("rows", "inner", "outer", "width"):
+                    assert kind is c_longlong, (name, parameter)
