@@ -11,6 +11,8 @@
 // warp one per lane, and a channel ten times larger than the others costs precision to its 31 neighbours only.
 //
 // Beside the largest number of a type, rounding up would leave the type: there the code below is taken (63 2^e, 240 2^e).
+// The pre-activations that a product's epilogue writes are FP32 values, within no 16-bit type's range: they are kept in FP32's
+// range and read by linear_dz_kernel alone.  A finite one beside 2^128 may read back as an infinity; slopes are at their limits there.
 // A group that holds an infinity or a NaN has the byte 255 and reads back as NaN throughout: a loss scaler sees it.
 // Codes behind the end of a row are zero.
 #pragma once

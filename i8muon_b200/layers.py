@@ -410,11 +410,14 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
 
     ``x`` (..., inner) in float16 or bfloat16, ``weight`` (outer, inner) as ``torch.nn.Linear`` holds it, ``bias`` (outer),
     ``residual`` (..., outer), all of one type.  ``activation``: None, "relu", "relu2" (max(z, 0)^2), "gelu" (with the
-    error function), "gelu_tanh" or "silu".  Sums, bias, activation and residual are FP32; the result is rounded once.
+    error function), "gelu_tanh" or "silu".  Sums, bias, activation and residual are FP32; the result is rounded once.  Logistic
+    functions below 2^-126 are zero: silu below -87.3, where it is -1e-36, and gelu_tanh below -10.
 
     For the backward pass ``x`` and, with an activation, the pre-activation rounded to the type of ``x`` are kept, or both in
     eight bits with ``checkpoint="int8"`` or ``"fp8"``.  The gradients are those of the formula at what was kept; the
-    gradient of the pre-activation is rounded to the type of ``x`` once, as the operand of the two backward products.
+    gradient of the pre-activation is rounded to the type of ``x`` once, as the operand of the two backward products.  A
+    pre-activation beyond the type of ``x`` is kept as an infinity (in eight bits within FP32's range); slopes there are 0 and 1,
+    and infinite on the right of relu2.
 
     A device-side wait that runs out is reported through the status word that ``check_status()`` and ``Muon.step()`` read; a
     first call on a device cannot be captured into a graph.  A backward pass is captured together with its forward pass, on
