@@ -3,7 +3,8 @@
 ``linear`` (bias, activation and residual in the product's epilogue), ``layer_norm``, and activations kept in eight bits for the backward pass (``quantise_activation``, ``restore_activation``,
 and the ``checkpoint=`` argument of the layers).  The functions take and return torch tensors, work on
 the current stream of the tensors' device without synchronising, and are differentiable once, in reverse mode; tensors that
-carry a tangent of forward mode are refused.  They run the sm_100a library's kernels; there is no fallback.  The reference starts at the gradient and has no counterpart.
+carry a tangent of forward mode are refused.  They run the sm_100a library's kernels; there is no fallback.  The reference
+starts at the gradient and has no counterpart.
 
 Eight-bit format: groups of 32 consecutive elements of a row share a power of two, the smallest 2^e with
 max|x| <= M 2^e (M = 127 for ``"int8"``, 448 for ``"fp8"``, E4M3; e >= -127), and each element is rounded to the nearest
@@ -367,10 +368,10 @@ class _Linear(torch.autograd.Function):
 def _linear_backward(ctx, dy):
     need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     activation, fmt, x_shape, w_shape, kept_z, x_offset, z_offset = ctx.settings
-    _refuse_tangents("linear", dy)
     dresidual = dy if need_r else None
     if not (need_x or need_w or need_b):
         return None, None, None, dresidual, None, None
+    _refuse_tangents("linear", dy)
     kept = iter(ctx.saved_tensors)
     weight = next(kept) if need_x else None
     x = next(kept) if need_w else None

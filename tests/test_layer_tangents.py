@@ -69,3 +69,16 @@ def test_a_tangent_of_the_results_gradient_is_refused(cuda_device, make):
             torch.autograd.grad(y, x, forward_ad.make_dual(dy, dy.clone()), retain_graph=True)
         got, = torch.autograd.grad(y, x, dy)
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_a_residuals_gradient_alone_keeps_its_tangent(cuda_device):
+    """It is the result's gradient itself: nothing is computed that could lose one."""
+    p = arguments(cuda_device)
+    r = p["x"].clone().requires_grad_()
+    y = linear(p["x"], p["w"], residual=r)
+    dy = torch.ones_like(y)
+    with forward_ad.dual_level():
+        got, = torch.autograd.grad(y, r, forward_ad.make_dual(dy, 2 * dy))
+        primal, tangent = forward_ad.unpack_dual(got)
+        assert torch.equal(primal, dy) and torch.equal(tangent, 2 * dy)
